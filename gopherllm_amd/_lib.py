@@ -16,6 +16,8 @@ TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_Q8_0, TYPE_Q4_K, TYPE_Q6_K = 0, 1, 30, 8, 12
 TYPE_Q4_0, TYPE_Q4_1, TYPE_Q2_K, TYPE_Q3_K, TYPE_Q5_K, TYPE_MXFP4 = 2, 3, 10, 11, 13, 39
 OK, EINVAL, EDEVICE, ENOMEM, EUNSUP = 0, -1, -2, -3, -4
 ATTN_EXACT, ATTN_SPLITK = 0, 1
+ROPE_INTERLEAVED, ROPE_HALF = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_YARN, ROPE_LLAMA3 = range(4)
 (T_WQ, T_WK, T_WV, T_WO, T_W1, T_W2, T_W3, T_TOK_EMBD, T_OUTPUT, T_ATTN_NORM, T_FFN_NORM,
  T_OUT_NORM) = range(12)
 
@@ -30,6 +32,13 @@ class ModelConfig(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("n_layers", "dim", "hidden", "n_heads", "n_kv_heads",
                                         "head_dim", "vocab", "max_len")] + [
         ("rms_eps", C.c_float), ("rope_theta", C.c_float)]
+
+
+class RopeConfig(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("head_dim", "rot_dim", "layout", "scaling", "orig_ctx")] + [
+        ("freq_factors", C.c_void_p)] + [
+        (n, C.c_double) for n in ("theta", "factor", "low_freq_factor", "high_freq_factor", "beta_fast",
+                                  "beta_slow", "attn_factor")]
 
 
 vp, i32, u32, u64, f32, sz = C.c_void_p, C.c_int, C.c_uint32, C.c_uint64, C.c_float, C.c_size_t
@@ -75,6 +84,19 @@ SIGNATURES = {
     "gllm_hip_kv_store_dev": (i32, [vp, i32, i32, vp, vp, vp]),
     "gllm_hip_attend_group": (i32, [vp, i32, i32, vp, i32, i32, i32, i32, i32, f32, f32, vp]),
     "gllm_hip_attend_dev": (i32, [vp, i32, vp, i32, i32, i32, i32, i32, f32, i32, vp, vp]),
+    "gllm_hip_rope_frequencies": (i32, [vp, vp, vp]),
+    "gllm_hip_rope_new": (vp, [vp]),
+    "gllm_hip_rope_release": (None, [vp]),
+    "gllm_hip_rope_dev": (i32, [vp, vp, i32, i32, i32, vp, vp, i32, vp]),
+    "gllm_hip_kv_store_rope_dev": (i32, [vp, i32, vp, vp, i32, i32, vp, i32, vp, i32, i32, i32, vp, vp, vp, i32, vp]),
+    "gllm_hip_attend_shared_bytes": (sz, [i32, i32, i32, i32, i32, i32]),
+    "gllm_hip_attend_shared_dev": (i32, [vp, i32, vp, i32, i32, i32, i32, i32, i32, vp, vp, i32, f32, vp, vp, sz, vp]),
+    "gllm_hip_attend_mass_bytes": (sz, [i32, i32, i32, i32, i32]),
+    "gllm_hip_attend_mass_dev": (i32, [vp, i32, vp, i32, i32, i32, i32, i32, i32, f32, vp, i32, vp, vp, sz, vp]),
+    "gllm_hip_kv_keep_bytes": (sz, [i32, i32, i32]),
+    "gllm_hip_kv_keep_dev": (i32, [vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, i32, vp, vp, i32, vp, vp, i32, vp,
+                                   sz, vp]),
+    "gllm_hip_kv_evict_store_dev": (i32, [vp, i32, i32, i32, vp, vp, i32, i32, i32, i32, vp, vp, i32, vp, vp, vp]),
     "gllm_hip_model_new": (vp, [vp]),
     "gllm_hip_model_release": (None, [vp]),
     "gllm_hip_model_set_weight": (i32, [vp, i32, i32, vp]),

@@ -12,6 +12,7 @@ C ABI (include/gllm_hip.h).  Names follow the Go API they stand in for:
     Weight.rows_dev          (Weight).RowInto           model.go:1034
     KVCacheF16.store_kv      (*KVCache).storeKV         model.go:1466
     KVCacheF16.attend_head_group (*KVCache).attendHeadGroup model.go:1516
+    Rope, KVCacheF16.store_rope_dev  prepareRopeScratch / applyPreparedRope model.go:3020-3093
 
 Host arrays are numpy; device arrays are torch tensors on a ROCm device (torch
 supplies device memory and streams only -- every computation is a HIP kernel
@@ -66,6 +67,37 @@ def _host_f32(a, numel: int, what: str):
     if a.size < numel:
         raise ValueError(f"{what}: {a.size} elements, need at least {numel}")
     return a
+
+
+def _dev_rows(t, kind: str, n: int, dim: int, what: str):
+    """(pointer, row stride) of n rows of at least dim values: a 1-D tensor of
+    one row, or a 2-D tensor whose rows are contiguous and may be apart."""
+    if not getattr(t, "is_cuda", False):
+        raise ValueError(f"{what}: expected a device tensor")
+    if str(t.dtype).replace("torch.", "") not in _DTYPES[kind]:
+        raise ValueError(f"{what}: dtype {t.dtype}, expected {kind}")
+    if t.dim() == 1:
+        t = t.unsqueeze(0)
+    if t.dim() != 2 or t.shape[0] != n or t.shape[1] < dim:
+        raise ValueError(f"{what}: shape {tuple(t.shape)}, need {n} rows of {dim}")
+    if t.shape[1] > 1 and t.stride(1) != 1 or n > 1 and t.stride(0) < dim:
+        raise ValueError(f"{what}: the values of a row must be contiguous, and rows must not overlap")
+    return _dev_ptr(t), t.stride(0) if n > 1 else t.shape[1]
+
+
+def _on_current_device(**tensors):
+    import torch
+    at = torch.cuda.current_device()
+    for what, t in tensors.items():
+        if t is not None and t.device.index != at:
+            raise ValueError(f"{what}: on device {t.device.index}, the current one is {at}")
+
+
+def _work(work):
+    """(pointer, bytes) of a caller's workspace, or of none."""
+    if work is None:
+        return None, 0
+    return _dev(work, "u8", 0, "work"), work.numel()
 
 
 def _rows(t):
@@ -299,6 +331,102 @@ def fill_normal_dev(out, seed: int, std: float, stream=None):
     return out
 
 
+class Rope:
+    """Rotary positions: head layout, part of the head and scaled frequencies
+    (buildRopeInvFreq model.go:1728-1799), kept on the current device.
+
+    layout: "interleaved" (pairs 2i, 2i + 1) or "half" (i, i + rot_dim / 2);
+    scaling: "none", "linear" (factor), "yarn" (factor, orig_ctx, beta_fast,
+    beta_slow) or "llama3" (factor, orig_ctx, low_freq_factor,
+    high_freq_factor); freq_factors: rot_dim / 2 divisors of the frequencies
+    (a GGUF file's rope_freqs.weight)."""
+
+    LAYOUTS = {"interleaved": _lib.ROPE_INTERLEAVED, "half": _lib.ROPE_HALF}
+    SCALINGS = {"none": _lib.ROPE_PLAIN, "linear": _lib.ROPE_LINEAR, "yarn": _lib.ROPE_YARN, "llama3": _lib.ROPE_LLAMA3}
+
+    def __init__(self, head_dim: int, rot_dim=None, layout="interleaved", theta: float = 500000.0, scaling="none",
+                 factor: float = 1.0, orig_ctx: int = 0, low_freq_factor: float = 1.0, high_freq_factor: float = 4.0,
+                 beta_fast: float = 32.0, beta_slow: float = 1.0, attn_factor: float = 1.0, freq_factors=None):
+        self.handle = None
+        cfg = self.config(head_dim, rot_dim, layout, theta, scaling, factor, orig_ctx, low_freq_factor, high_freq_factor,
+                          beta_fast, beta_slow, attn_factor, freq_factors)
+        self.head_dim, self.rot_dim = cfg.head_dim, cfg.rot_dim
+        self.handle = call_ptr("gllm_hip_rope_new", C.byref(cfg))
+
+    @classmethod
+    def config(cls, head_dim, rot_dim=None, layout="interleaved", theta=500000.0, scaling="none", factor=1.0, orig_ctx=0,
+               low_freq_factor=1.0, high_freq_factor=4.0, beta_fast=32.0, beta_slow=1.0, attn_factor=1.0,
+               freq_factors=None):
+        if layout not in cls.LAYOUTS or scaling not in cls.SCALINGS:
+            raise ValueError(f"Rope: layout {layout!r}, scaling {scaling!r}")
+        c = _lib.RopeConfig()
+        c.head_dim, c.rot_dim = int(head_dim), int(head_dim if rot_dim is None else rot_dim)
+        c.layout, c.scaling, c.orig_ctx = cls.LAYOUTS[layout], cls.SCALINGS[scaling], int(orig_ctx)
+        c.theta, c.factor, c.attn_factor = float(theta), float(factor), float(attn_factor)
+        c.low_freq_factor, c.high_freq_factor = float(low_freq_factor), float(high_freq_factor)
+        c.beta_fast, c.beta_slow = float(beta_fast), float(beta_slow)
+        if freq_factors is not None:
+            c._kept = _host_f32(freq_factors, c.rot_dim // 2, "Rope freq_factors")
+            c.freq_factors = c._kept.ctypes.data
+        return c
+
+    @classmethod
+    def frequencies(cls, *args, **kwargs):
+        """(inverse frequencies, amplitude) of a configuration, in 64 bits; on the host."""
+        c = cls.config(*args, **kwargs)
+        inv, amp = np.empty(max(0, c.rot_dim // 2), np.float64), C.c_double(0)
+        call("gllm_hip_rope_frequencies", C.byref(c), _np_ptr(inv), C.byref(amp))
+        return inv, amp.value
+
+    def apply_dev(self, x, positions, out=None, stream=None):
+        """Rotate x (tokens, heads * head_dim) by positions (int32), in place without out."""
+        out = x if out is None else out
+        n = positions.numel()
+        _on_current_device(x=x, positions=positions, out=out)
+        heads = x.shape[-1] // self.head_dim
+        if heads * self.head_dim != x.shape[-1]:
+            raise ValueError(f"x: rows of {x.shape[-1]} are not heads of {self.head_dim}")
+        xp, xs = _dev_rows(x, "f32", n, heads * self.head_dim, "x")
+        op, os = _dev_rows(out, "f32", n, heads * self.head_dim, "out")
+        call("gllm_hip_rope_dev", self.handle, xp, xs, n, heads, _dev(positions, "i32", n, "positions"), op, os,
+             _stream(stream))
+        return out
+
+    def release(self):
+        if self.handle:
+            load().gllm_hip_rope_release(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.release()
+        except Exception:
+            pass
+
+
+def attend_shared_bytes(n, n_heads, n_kv_heads, hd, length, most) -> int:
+    """Bytes of a workspace for KVCacheF16.attend_shared_dev."""
+    return int(load().gllm_hip_attend_shared_bytes(n, n_heads, n_kv_heads, hd, length, most))
+
+
+def attend_mass_bytes(n, n_heads, n_kv_heads, hd, length) -> int:
+    """Bytes of a workspace for KVCacheF16.attend_mass_dev over `length` rows."""
+    return int(load().gllm_hip_attend_mass_bytes(n, n_heads, n_kv_heads, hd, length))
+
+
+def keep_bytes(layers, n_kv_heads, budget) -> int:
+    """Bytes of a workspace for KVCacheF16.keep_dev."""
+    return int(load().gllm_hip_kv_keep_bytes(layers, n_kv_heads, budget))
+
+
+class _DeviceRows:
+    """A cache's rows for torch.as_tensor, which keeps this object (and the cache) alive."""
+
+    def __init__(self, cache, ptr, rows, dim):
+        self.cache = cache
+        self.__cuda_array_interface__ = {"shape": (rows, dim), "typestr": "<f2", "data": (ptr, False), "version": 2}
+
+
 class KVCacheF16:
     """HBM-resident F16 KV cache (NewKVCacheF16, model.go:1396)."""
 
@@ -354,3 +482,89 @@ class KVCacheF16:
              n_kv_heads, hd, start, end, scale, mode, _dev(out, "f32", n_heads * hd, "out"),
              _stream(stream))
         return out
+
+    def tensors(self, layer):
+        """(K, V) of a layer as float16 tensors of max_len rows over the cache's own memory."""
+        import torch
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"tensors: layer {layer} of {self.layers}")
+        return tuple(torch.as_tensor(_DeviceRows(self, p, self.max_len, d), device="cuda")
+                     for p, d in ((self.k_ptr(layer), self.kv_dim_k), (self.v_ptr(layer), self.kv_dim_v)))
+
+    def store_rope_dev(self, layer, rope: Rope, q, k, v, positions, rows, q_out=None, stream=None):
+        """Rotate q (tokens, heads * hd; or None) into q_out (default: in place) and
+        k (tokens, kv heads * hd) by positions, and store k and v as f16 in the
+        cache's rows (int32; outside the cache: not stored; all different)."""
+        n, hd = positions.numel(), rope.head_dim
+        q_out = q if q_out is None else q_out
+        _on_current_device(q=q, k=k, v=v, positions=positions, rows=rows, q_out=q_out)
+        heads, n_kv = (0 if q is None else q.shape[-1] // hd), k.shape[-1] // hd
+        if k.shape[-1] != n_kv * hd or v.shape[-1] != k.shape[-1] or q is not None and q.shape[-1] != heads * hd:
+            raise ValueError(f"store_rope_dev: q, k or v rows are not heads of {hd}")
+        qp, qs = (None, 0) if q is None else _dev_rows(q, "f32", n, heads * hd, "q")
+        op, os = (None, 0) if q is None else _dev_rows(q_out, "f32", n, heads * hd, "q_out")
+        kp, ks = _dev_rows(k, "f32", n, n_kv * hd, "k")
+        vp, vs = _dev_rows(v, "f32", n, n_kv * hd, "v")
+        call("gllm_hip_kv_store_rope_dev", self.handle, layer, rope.handle, qp, qs, heads, kp, ks, vp, vs, n_kv, n,
+             _dev(positions, "i32", n, "positions"), _dev(rows, "i32", n, "rows"), op, os, _stream(stream))
+        return q_out
+
+    def attend_shared_dev(self, layer, q, n_heads, n_kv_heads, hd, start, length, starts, lens, most, scale, out,
+                          work=None, stream=None):
+        """One token of each request: q (requests, n_heads * hd) over the shared rows
+        start .. start + length - 1 and, with most > 0, its own lens[i] rows from
+        starts[i] (int32 tensors; most: the length the work is split for)."""
+        n = q.shape[0] if q.dim() > 1 else 1
+        _on_current_device(q=q, starts=starts, lens=lens, out=out, work=work)
+        wp, wb = _work(work)
+        call("gllm_hip_attend_shared_dev", self.handle, layer, _dev(q, "f32", n * n_heads * hd, "q"), n, n_heads,
+             n_kv_heads, hd, start, length, None if starts is None else _dev(starts, "i32", n, "starts"),
+             None if lens is None else _dev(lens, "i32", n, "lens"), most, scale,
+             _dev(out, "f32", n * n_heads * hd, "out"), wp, wb, _stream(stream))
+        return out
+
+    def attend_mass_dev(self, layer, q, n_heads, n_kv_heads, hd, start, end, scale, mass, out, work=None, stream=None):
+        """The newest tokens q (tokens, n_heads * hd), the last at row `end`, causally over
+        rows start .. end; each row's weight is added to mass (n_kv_heads, >= end + 1)."""
+        n = q.shape[0] if q.dim() > 1 else 1
+        _on_current_device(q=q, mass=mass, out=out, work=work)
+        wp, wb = _work(work)
+        stride = mass.shape[-1]
+        call("gllm_hip_attend_mass_dev", self.handle, layer, _dev(q, "f32", n * n_heads * hd, "q"), n, n_heads,
+             n_kv_heads, hd, start, end, scale, _dev(mass, "f32", n_kv_heads * stride, "mass"), stride,
+             _dev(out, "f32", n * n_heads * hd, "out"), wp, wb, _stream(stream))
+        return out
+
+    def keep_dev(self, dst: "KVCacheF16", n_kv_heads, hd, length, budget, mass, pos, mass_out, pos_out, now, sinks=0,
+                 recent=0, start=0, dst_start=0, work=None, stream=None):
+        """Copy the budget rows of most mass (positions < sinks or >= now - recent first)
+        of rows start .. start + length - 1, per layer and kv head, to dst from
+        dst_start on.  mass, pos (or None: the row): (layers, n_kv_heads, rows of this
+        cache); mass_out, pos_out: (layers, n_kv_heads, rows of dst)."""
+        _on_current_device(mass=mass, pos=pos, mass_out=mass_out, pos_out=pos_out, work=work)
+        stride, out_stride = mass.shape[-1], mass_out.shape[-1]
+        if pos is not None and pos.shape[-1] != stride or pos_out.shape[-1] != out_stride:
+            raise ValueError("keep_dev: mass and pos rows of different lengths")
+        n = self.layers * n_kv_heads
+        wp, wb = _work(work)
+        call("gllm_hip_kv_keep_dev", self.handle, dst.handle, n_kv_heads, hd, start, length, dst_start, budget, sinks,
+             recent, now, _dev(mass, "f32", n * stride, "mass"),
+             None if pos is None else _dev(pos, "i32", n * stride, "pos"), stride,
+             _dev(mass_out, "f32", n * out_stride, "mass_out"), _dev(pos_out, "i32", n * out_stride, "pos_out"),
+             out_stride, wp, wb, _stream(stream))
+
+    def evict_store_dev(self, layer, n_kv_heads, hd, k, v, start, length, mass, pos, now, sinks=0, recent=0,
+                        rows_out=None, stream=None):
+        """Store a token's k and v (n_kv_heads * hd, rotated) per kv head in place of the
+        unprotected row of least mass among start .. start + length - 1; its pos
+        becomes now (an int32 device tensor of one value), its mass 0.  mass, pos:
+        (n_kv_heads, rows); rows_out: n_kv_heads int32, the rows given up."""
+        _on_current_device(k=k, v=v, mass=mass, pos=pos, now=now, rows_out=rows_out)
+        stride = mass.shape[-1]
+        if pos.shape[-1] != stride:
+            raise ValueError("evict_store_dev: mass and pos rows of different lengths")
+        call("gllm_hip_kv_evict_store_dev", self.handle, layer, n_kv_heads, hd, _dev(k, "f32", n_kv_heads * hd, "k"),
+             _dev(v, "f32", n_kv_heads * hd, "v"), start, length, sinks, recent,
+             _dev(mass, "f32", n_kv_heads * stride, "mass"), _dev(pos, "i32", n_kv_heads * stride, "pos"), stride,
+             _dev(now, "i32", 1, "now"), None if rows_out is None else _dev(rows_out, "i32", n_kv_heads, "rows_out"),
+             _stream(stream))

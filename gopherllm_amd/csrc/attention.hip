@@ -17,6 +17,7 @@
 #include <cstdlib>
 
 #include "attn_exp.h"
+#include "kv_cache.h"
 
 namespace gllm {
 size_t attend_prefill_floats(int p, int n_heads, int n_kv, int span_max);
@@ -40,17 +41,6 @@ __device__ __forceinline__ void exp_row(float* row, int first, int stride, int s
             if (t0 + i * stride < span) row[t0 + i * stride] = ev[i];
     }
 }
-
-}  // namespace gllm
-
-struct gllm_hip_kv {
-    int layers, kv_dim_k, kv_dim_v, max_len;
-    uint16_t** k;  // host array of device pointers
-    uint16_t** v;
-    int device;
-};
-
-namespace gllm {
 
 __global__ void kv_store_kernel(const float* __restrict__ k, const float* __restrict__ v,
                                 uint16_t* __restrict__ kd, uint16_t* __restrict__ vd, int nk,

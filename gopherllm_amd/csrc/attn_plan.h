@@ -1,0 +1,81 @@
+// attn_plan.h -- how attention over cache ranges is split over workgroups and
+// what its workspace holds.  Host arithmetic only, so it is tested without a device.
+#pragma once
+
+#include <stddef.h>
+
+#include <algorithm>
+
+namespace gllm {
+
+constexpr int kSeqWaves = 4;                  // waves of a workgroup, each with a run of positions
+constexpr int kSeqTile = 32;                  // positions of a wave's step
+constexpr int kSeqQuantum = kSeqWaves * kSeqTile;
+constexpr int kSeqTarget = 512;               // workgroups: two for each of the 256 CUs
+constexpr int kSeqMaxSplits = 64;             // partial results of a query row from one range
+
+// Query rows of a kv head: n tokens x r heads, in blocks of 16 * nq rows.
+struct SeqPlan {
+    int r;                    // query heads of a kv head
+    int nq, row_blocks;       // of the shared range
+    int chunk, chunks;        // positions of a workgroup, workgroups per row block
+    int own_blocks, splits;   // of each token's own range (16 rows a block)
+    int slots;                // partial results of a query row
+    size_t rows;              // n * n_heads
+};
+
+inline int ceil_div(int a, int b) { return (int)(((long long)a + b - 1) / b); }
+
+// n tokens, heads / kv heads, `len` shared positions, own ranges planned for
+// `most` positions (0: none).
+inline SeqPlan seq_plan(int n, int n_heads, int n_kv, int len, int most) {
+    SeqPlan p{};
+    p.r = n_heads / n_kv;
+    p.rows = (size_t)n * n_heads;
+    const long long per_kv = (long long)n * p.r;
+    p.nq = per_kv <= 16 ? 1 : per_kv <= 32 ? 2 : 4;
+    p.row_blocks = (int)((per_kv + 16 * p.nq - 1) / (16 * p.nq));
+    if (len > 0) {
+        const long long per_chunk = (long long)n_kv * p.row_blocks;
+        const int want = (int)std::max(1LL, std::min((long long)kSeqMaxSplits, kSeqTarget / per_chunk));
+        p.chunk = ceil_div(ceil_div(len, want), kSeqQuantum) * kSeqQuantum;
+        p.chunks = ceil_div(len, p.chunk);
+    }
+    if (most > 0) {
+        p.own_blocks = ceil_div(p.r, 16);
+        const long long per_split = (long long)n * n_kv * p.own_blocks;
+        const int want = (int)std::max(1LL, std::min((long long)kSeqMaxSplits, kSeqTarget / per_split));
+        p.splits = std::min(want, ceil_div(most, kSeqQuantum));
+    }
+    p.slots = p.chunks + p.splits;
+    return p;
+}
+
+// Floats of the workspace: base and sum of every partial result, its output,
+// and for `scored` positions the scores of every row with the row's final
+// base and 1 / sum.
+inline size_t seq_floats(const SeqPlan& p, int hd, size_t scored) {
+    const size_t parts = p.rows * (size_t)p.slots;
+    size_t f = parts * (2 + (size_t)hd);
+    if (scored) f += p.rows * (scored + 2);
+    return f + 64;
+}
+
+// Rows a .. b - 1 of a cache of max_len rows that the range start, len names.
+struct RowSpan {
+    int a, b;
+};
+#ifdef __HIPCC__
+__host__ __device__
+#endif
+inline RowSpan clip_rows(int start, int len, int max_len) {
+    const long long lo = start < 0 ? 0 : start;
+    long long hi = (long long)start + (len < 0 ? 0 : len);
+    if (hi > max_len) hi = max_len;
+    RowSpan s;
+    s.a = lo > max_len ? max_len : (int)lo;
+    s.b = hi < s.a ? s.a : (int)hi;
+    return s;
+}
+
+}  // namespace gllm

@@ -269,6 +269,114 @@ int gllm_hip_attend_dev(gllm_hip_kv* kv, int l, const float* d_q, int n_heads, i
                         void* stream);
 
 /* ---------------------------------------------------------------------- */
+/* Rotary positions, batches and bounds of the F16 KV cache.  A cache is    */
+/* rows that any position of any request may take: the keys carry their    */
+/* rotation with them, and attention does not depend on the order of rows. */
+/* The reference rotates inside its graph (applyPreparedRope               */
+/* model.go:3051), attends one sequence at a time and ends at max_len.     */
+/*                                                                         */
+/* Workspaces: a call that takes d_work / work_bytes works in that device   */
+/* buffer (16-byte aligned, at least the bytes its _bytes function says),  */
+/* or, with d_work null, in the calling thread's scratch for the stream.   */
+/* Graphs captured on one stream with null share that scratch and must not */
+/* be replayed at the same time; with a d_work each they may.  Caches,      */
+/* ropes and tensors must be on the current device (GLLM_EINVAL).          */
+/* ---------------------------------------------------------------------- */
+
+#define GLLM_ROPE_INTERLEAVED 0 /* pairs (2i, 2i + 1) (ropeInterleaved model.go:3084) */
+#define GLLM_ROPE_HALF 1        /* pairs (i, i + rot_dim / 2) */
+
+#define GLLM_ROPE_PLAIN 0
+#define GLLM_ROPE_LINEAR 1 /* every frequency / factor */
+#define GLLM_ROPE_YARN 2   /* model.go:1758-1799: factor, orig_ctx, beta_fast, beta_slow */
+#define GLLM_ROPE_LLAMA3 3 /* factor, orig_ctx, low_freq_factor, high_freq_factor */
+
+typedef struct gllm_hip_rope_config {
+    int head_dim, rot_dim; /* the first rot_dim (even) values of a head turn, the others stay */
+    int layout, scaling;
+    int orig_ctx;
+    const float* freq_factors; /* null, or rot_dim / 2 divisors (rope_freqs.weight) */
+    double theta, factor, low_freq_factor, high_freq_factor, beta_fast, beta_slow;
+    double attn_factor; /* amplitude of the rotated values; yarn multiplies it by 0.1 ln(factor) + 1 */
+} gllm_hip_rope_config;
+
+typedef struct gllm_hip_rope gllm_hip_rope;
+
+/* The rot_dim / 2 inverse frequencies and the amplitude (host only). */
+int gllm_hip_rope_frequencies(const gllm_hip_rope_config* cfg, double* inv, double* amp);
+/* The same frequencies on the current device. */
+gllm_hip_rope* gllm_hip_rope_new(const gllm_hip_rope_config* cfg);
+void gllm_hip_rope_release(gllm_hip_rope* r);
+/* Rotate the heads of n tokens: d_x and d_out are rows of heads * head_dim
+ * floats, x_stride and out_stride apart; token t turns by d_pos[t].  d_out may
+ * be d_x (with the same stride) and must not overlap it otherwise.  Angles are
+ * 64-bit products, right to float32 for every int32 position. */
+int gllm_hip_rope_dev(const gllm_hip_rope* r, const float* d_x, int x_stride, int n, int heads,
+                      const int32_t* d_pos, float* d_out, int out_stride, void* stream);
+/* The same for the queries and keys of n tokens, with the store: rotated keys
+ * and values are rounded to f16 (RNE) into row d_rows[t] of layer l.  A row
+ * outside 0..max_len-1 (such as -1, padding) is not stored; the rows of a call
+ * must differ (of two tokens that share one, either may end up in any part of
+ * it).  d_q may be null: keys and values only. */
+int gllm_hip_kv_store_rope_dev(gllm_hip_kv* kv, int l, const gllm_hip_rope* r, const float* d_q,
+                               int q_stride, int n_heads, const float* d_k, int k_stride,
+                               const float* d_v, int v_stride, int n_kv_heads, int n,
+                               const int32_t* d_pos, const int32_t* d_rows, float* d_q_out,
+                               int out_stride, void* stream);
+
+/* Decode attention of n requests, one token each (d_q [n][n_heads][hd] ->
+ * d_out, 16-byte aligned; hd % 8 == 0, hd <= 128; kv_dim % 8 == 0): request i
+ * attends the shared rows start .. start + len - 1, read once for the whole
+ * batch, and its own rows d_starts[i] .. d_starts[i] + d_lens[i] - 1 (device
+ * arrays, cut to the cache; a length <= 0 is none).  `most` is the own length
+ * that the work is split for; longer ranges are attended whole too.  most 0
+ * with null arrays: no own rows, as for cross attention to an encoder's
+ * states.  Ranges may overlap: several tokens of one request are several
+ * requests whose own ranges start together (a row in both ranges counts
+ * twice).  A request without any row gets zeros.  Sums are float32, products
+ * of 22-bit q and weights; where an attended row holds an infinity or NaN the
+ * outputs of its kv head are not finite. */
+size_t gllm_hip_attend_shared_bytes(int n, int n_heads, int n_kv_heads, int hd, int len, int most);
+int gllm_hip_attend_shared_dev(gllm_hip_kv* kv, int l, const float* d_q, int n, int n_heads,
+                               int n_kv_heads, int hd, int start, int len,
+                               const int32_t* d_starts, const int32_t* d_lens, int most,
+                               float scale, float* d_out, void* d_work, size_t work_bytes,
+                               void* stream);
+/* Attention of the n newest tokens of one sequence (d_q [n][n_heads][hd]):
+ * token i attends rows start .. end - (n - 1) + i.  d_mass [n_kv_heads]
+ * [mass_stride] floats: the weight that row t received from all tokens and
+ * the heads of a kv head is added to d_mass[g][t].  Otherwise as above. */
+size_t gllm_hip_attend_mass_bytes(int n, int n_heads, int n_kv_heads, int hd, int len);
+int gllm_hip_attend_mass_dev(gllm_hip_kv* kv, int l, const float* d_q, int n, int n_heads,
+                             int n_kv_heads, int hd, int start, int end, float scale,
+                             float* d_mass, int mass_stride, float* d_out, void* d_work,
+                             size_t work_bytes, void* stream);
+/* Copy the `budget` rows that matter most of src rows start .. start + len - 1
+ * to dst rows dst_start .. , in every layer and for every kv head on its own,
+ * in row order.  Rows whose position is < sinks or >= now - recent come first
+ * (now: the position of the next token), all alike, then those of most mass;
+ * NaN is below every number; of equals, the lowest rows stay.  d_mass and d_pos: [layers]
+ * [n_kv_heads][stride], indexed by row (d_pos null: a row is its position);
+ * the kept rows' values go to d_mass_out and d_pos_out [layers][n_kv_heads]
+ * [out_stride] at their new rows.  dst is another cache, of as many layers;
+ * outputs must not overlap the inputs. */
+size_t gllm_hip_kv_keep_bytes(int layers, int n_kv_heads, int budget);
+int gllm_hip_kv_keep_dev(const gllm_hip_kv* src, gllm_hip_kv* dst, int n_kv_heads, int hd,
+                         int start, int len, int dst_start, int budget, int sinks, int recent,
+                         int now, const float* d_mass, const int32_t* d_pos, int stride,
+                         float* d_mass_out, int32_t* d_pos_out, int out_stride, void* d_work,
+                         size_t work_bytes, void* stream);
+/* A decode step of a bounded cache: per kv head, the row of start .. start +
+ * len - 1 that comes last in that order (of equals, the lowest) takes the new token's key and value
+ * (d_k, d_v: n_kv_heads * hd floats, rotated already), position *d_now
+ * (device) and mass 0.  d_mass and d_pos: [n_kv_heads][stride], indexed by
+ * row.  d_rows_out, if set: the row each kv head gave up. */
+int gllm_hip_kv_evict_store_dev(gllm_hip_kv* kv, int l, int n_kv_heads, int hd, const float* d_k,
+                                const float* d_v, int start, int len, int sinks, int recent,
+                                float* d_mass, int32_t* d_pos, int stride, const int32_t* d_now,
+                                int32_t* d_rows_out, void* stream);
+
+/* ---------------------------------------------------------------------- */
 /* Resident llama decoder (ForwardBodyInto model.go:2622,                  */
 /* ForwardBatchInto forward_batch.go:316, forwardGreedyToken               */
 /* runtime.go:1607)                                                        */
