@@ -8,16 +8,15 @@
 
 namespace gllm {
 
-constexpr int kSeqWaves = 4;                  // waves of a workgroup, each with a run of positions
-constexpr int kSeqTile = 32;                  // positions of a wave's step
-constexpr int kSeqQuantum = kSeqWaves * kSeqTile;
+constexpr int kSeqWaves = 4;                  // waves of a workgroup
+constexpr int kSeqQuantum = 128;              // positions: one step of every shape of workgroup, or more
 constexpr int kSeqTarget = 512;               // workgroups: two for each of the 256 CUs
 constexpr int kSeqMaxSplits = 64;             // partial results of a query row from one range
 
-// Query rows of a kv head: n tokens x r heads, in blocks of 16 * nq rows.
+// Query rows of a kv head: n tokens x r heads.
 struct SeqPlan {
     int r;                    // query heads of a kv head
-    int nq, row_blocks;       // of the shared range
+    int nq, rw, row_blocks;   // of the shared range: blocks of 16 nq rw rows, over rw waves
     int chunk, chunks;        // positions of a workgroup, workgroups per row block
     int own_blocks, splits;   // of each token's own range (16 rows a block)
     int slots;                // partial results of a query row
@@ -33,8 +32,9 @@ inline SeqPlan seq_plan(int n, int n_heads, int n_kv, int len, int most) {
     p.r = n_heads / n_kv;
     p.rows = (size_t)n * n_heads;
     const long long per_kv = (long long)n * p.r;
-    p.nq = per_kv <= 16 ? 1 : per_kv <= 32 ? 2 : 4;
-    p.row_blocks = (int)((per_kv + 16 * p.nq - 1) / (16 * p.nq));
+    p.nq = per_kv <= 16 ? 1 : 2;
+    p.rw = per_kv <= 32 ? 1 : per_kv <= 64 ? 2 : 4;
+    p.row_blocks = (int)((per_kv + 16 * p.nq * p.rw - 1) / (16 * p.nq * p.rw));
     if (len > 0) {
         const long long per_chunk = (long long)n_kv * p.row_blocks;
         const int want = (int)std::max(1LL, std::min((long long)kSeqMaxSplits, kSeqTarget / per_chunk));

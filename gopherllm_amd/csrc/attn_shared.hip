@@ -15,12 +15,12 @@
 // first scaled by a power of two to a maximum in [2^14, 2^15), and the
 // weights by 2^15 (the 15 in base), so that the second part stays normal.
 //
-// A workgroup's four waves split the positions of a chunk.  Per 32 positions
-// a wave forms the transposed scores S^T = K Q^T and the transposed output
+// A workgroup's four waves split the positions of a chunk, or its query rows
+// where there are many.  Per 32 positions a wave forms the transposed scores S^T = K Q^T and the transposed output
 // O^T += V^T W^T: the accumulator layout of S^T (query = lane & 15, position
 // = 4 * (lane / 16) + register) is, for two tiles of 16 positions, the
 // operand layout of W^T, so the weights never leave the lane.  V^T is read
-// from a wave's own LDS tile with the transposing loads.
+// from an LDS tile with the transposing loads.
 #include <algorithm>
 
 #include "attn_plan.h"
@@ -47,7 +47,8 @@ struct SeqArgs {
     const int32_t* starts;  // own rows
     const int32_t* lens;
     int own_blocks, splits;
-    int slot0, slots;     // first partial of this launch, partials per row
+    int shared_wgs;       // workgroups of the shared range
+    int slot0, slots;     // first partial of the own ranges, partials per row
     float scale;          // scale * log2(e)
     float* pm;            // [row][slot] base
     float* pl;            //             sum
@@ -58,32 +59,56 @@ struct SeqArgs {
 
 constexpr float kSeqLift = 15.0f;
 
-// XOR on the 16-byte chunk index of V row r, so that the four rows that a
-// 16-lane group of a transposing load reads lie in different banks.
+// Bytes between rows of an LDS tile.  K rows are read 16 bytes a lane, eight
+// rows at a time: 16 bytes of padding spread them over the banks.  V rows are
+// read 32 bytes a row, four rows at a time, by the transposing loads: rows of
+// 256 and 128 bytes need 32 bytes of padding, 192 and 64 spread by themselves.
 template <int HD>
-__device__ __forceinline__ int v_swizzle(int r) {
-    if (HD == 128) return 2 * (r & 3);
-    if (HD == 64) return 2 * ((r >> 1) & 1);
-    return 0;  // 192- and 64-byte rows spread by themselves
+struct Lds {
+    static constexpr int k_row = HD * 2 + 16;
+    static constexpr int v_row = HD * 2 + (HD % 64 == 0 ? 32 : 0);
+};
+
+template <int HD, int NQ, int RW>
+struct SeqShape {
+    static constexpr int PW = kSeqWaves / RW;                // position groups
+    static constexpr int STEP = RW == 4 ? 64 : 32;           // positions of a step
+    static constexpr int TILE = STEP * ((RW > 1 ? Lds<HD>::k_row : 0) + Lds<HD>::v_row);
+    static constexpr int BUFS = RW > 1 ? 2 : 1;
+    static constexpr int MERGE = PW > 1 ? kSeqWaves * 16 * (HD + 4) * 4 : 0;
+    static constexpr int BYTES = PW * BUFS * TILE > MERGE ? PW * BUFS * TILE : MERGE;
+};
+
+__device__ __forceinline__ h8 join(s4 a, s4 b) {
+    h8 r;
+    const h4 x = __builtin_bit_cast(h4, a), y = __builtin_bit_cast(h4, b);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        r[j] = x[j];
+        r[4 + j] = y[j];
+    }
+    return r;
 }
 
 // HD: head size rounded up to 32 (hd <= HD, hd % 8 == 0); NQ: tiles of 16
-// query rows; OWN: each token's own rows instead of the shared ones.
-template <int HD, int NQ, bool OWN>
-__global__ __launch_bounds__(256) void seq_attend_kernel(SeqArgs a) {
-    constexpr int KK = HD / 32, DT = HD / 16, CH = HD / 8;
-    constexpr int VB = kSeqTile * HD;  // halves of a V tile
-    __shared__ __align__(16) _Float16 vs[kSeqWaves][VB];
-    __shared__ __align__(16) float so[kSeqWaves][16][HD];
-    __shared__ float sm[kSeqWaves][16], sl[kSeqWaves][16];
+// query rows of a wave; RW: waves that take different query rows over the same
+// positions, sharing the K and V tiles; the kSeqWaves / RW groups of such waves
+// take different positions.  OWN: each token's own rows, not the shared ones.
+template <int HD, int NQ, int RW, bool OWN>
+__device__ __forceinline__ void seq_run(const SeqArgs& a, int b, char* lds, float (*sm)[16], float (*sl)[16]) {
+    using S = SeqShape<HD, NQ, RW>;
+    constexpr int KK = HD / 32, DT = HD / 16, CH = HD / 8, PW = S::PW, STEP = S::STEP, ST = STEP / 16;
+    constexpr int GT = RW * 64;                    // threads of a position group
+    constexpr int LD = STEP * CH / GT;             // 16-byte loads of a thread for a tile
+    static_assert(STEP * CH % GT == 0, "a tile is a whole number of loads");
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int col = lane & 15, grp = lane >> 4;
+    const int pg = wave / RW, rw = wave % RW;
     const float ninf = -__int_as_float(0x7f800000);
 
-    int g, rb, slot, tok = 0, a0, a1;  // rows a0 .. a1 - 1 of the cache
-    int b = blockIdx.x;
-    g = b % a.n_kv;
+    const int g = b % a.n_kv;
     b /= a.n_kv;
+    int rb, slot, tok = 0, a0, a1;  // rows a0 .. a1 - 1 of the cache
     if (OWN) {
         rb = b % a.own_blocks;
         b /= a.own_blocks;
@@ -99,40 +124,35 @@ __global__ __launch_bounds__(256) void seq_attend_kernel(SeqArgs a) {
         a0 = a.start + slot * a.chunk;
         a1 = min(a.start + a.len, a0 + a.chunk);
     }
-    const int part = ((a1 - a0 + kSeqQuantum - 1) / kSeqQuantum) * kSeqTile;  // positions of a wave
-    const int p0 = min(a1, a0 + wave * part), p1 = min(a1, p0 + part);
+    const int part = ((a1 - a0 + PW * STEP - 1) / (PW * STEP)) * STEP;  // positions of a group
+    const int p0 = min(a1, a0 + pg * part), p1 = min(a1, p0 + part);
 
-    // query rows: row = rb * 16 * NQ + 16 * nq + col of this kv head
+    // query rows: rb * 16 * NQ * RW + 16 * (rw * NQ + nq) + col of this kv head
     const int rows = OWN ? a.r : a.n * a.r;
+    const int row0 = (rb * RW + rw) * 16 * NQ;
     h8 qh[NQ][KK], ql[NQ][KK];
     float c[NQ];
-    int lim[NQ];  // rows past it are masked
-    size_t part_row[NQ];
+    int lim[NQ];  // rows from it on are masked
 #pragma unroll
     for (int nq = 0; nq < NQ; nq++) {
-        const int rr = rb * 16 * NQ + 16 * nq + col;
+        const int rr = row0 + 16 * nq + col;
         const bool on = rr < rows;
         const int i = OWN ? tok : rr / a.r, hh = OWN ? rr : rr - i * a.r;
         const size_t row = on ? (size_t)i * a.n_heads + g * a.r + hh : 0;
-        part_row[nq] = row;
-        lim[nq] = a.causal ? a.start + a.len - (a.n - 1 - (on ? i : 0)) : a1;
-        float x[KK][8];
+        lim[nq] = a.causal ? min(p1, a.start + a.len - (a.n - 1 - (on ? i : 0))) : p1;
+        f4 x[KK][2];
         float mx = 0.0f;
 #pragma unroll
         for (int kk = 0; kk < KK; kk++) {
             const int d = 32 * kk + 8 * grp;
-            f4 u = {0, 0, 0, 0}, v = {0, 0, 0, 0};
+            x[kk][0] = x[kk][1] = f4{0, 0, 0, 0};
             if (on && d < a.hd) {
                 const float* p = a.q + row * a.hd + d;
-                u = *(const f4*)p;
-                v = *(const f4*)(p + 4);
+                x[kk][0] = *(const f4*)p;
+                x[kk][1] = *(const f4*)(p + 4);
             }
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                x[kk][j] = u[j];
-                x[kk][4 + j] = v[j];
-                mx = fmaxf(mx, fmaxf(fabsf(u[j]), fabsf(v[j])));
-            }
+            for (int j = 0; j < 4; j++) mx = fmaxf(mx, fmaxf(fabsf(x[kk][0][j]), fabsf(x[kk][1][j])));
         }
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
@@ -140,17 +160,19 @@ __global__ __launch_bounds__(256) void seq_attend_kernel(SeqArgs a) {
         int e = 15;
         if (mx > 0.0f && mx < __int_as_float(0x7f800000)) (void)frexpf(mx, &e);
         const int k = 15 - e;
-        c[nq] = ldexpf(a.scale, -k);
+        c[nq] = ldexpf(fabsf(a.scale), -k);  // the sign goes into q, so a larger dot is a larger score
 #pragma unroll
         for (int kk = 0; kk < KK; kk++)
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float v = ldexpf(x[kk][j], k);
+                const float v = ldexpf(a.scale < 0.0f ? -x[kk][j >> 2][j & 3] : x[kk][j >> 2][j & 3], k);
                 const _Float16 hi = (_Float16)v;
                 qh[nq][kk][j] = hi;
                 ql[nq][kk][j] = (_Float16)(v - (float)hi);
             }
     }
+    int lim_all = a1;  // rows that no row of this wave masks
+    if (!OWN && a.causal) lim_all = a.start + a.len - (a.n - 1 - min(row0 / a.r, a.n - 1));
 
     f4 o[NQ][DT];
     float base[NQ], l[NQ];
@@ -161,171 +183,306 @@ __global__ __launch_bounds__(256) void seq_attend_kernel(SeqArgs a) {
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) o[nq][dt] = f4{0, 0, 0, 0};
     }
-    _Float16* vt = vs[wave];
-    for (int pb = p0; pb < p1; pb += kSeqTile) {
-        // K operands: position 16 t + col, 8 dims at 32 kk + 8 grp
-        h8 kf[2][KK];
+
+    // a tile's K and V as loads: RW > 1: chunk e = GT u + thread of the group,
+    // to LDS; RW == 1: K straight into operand order
+    const uint16_t* Kg = a.K + g * a.hd;
+    const uint16_t* Vg = a.V + g * a.hd;
+    const bool whole = a.hd == HD;
+    const int gt = rw * 64 + lane;
+    u4 kr[LD], vr[LD];
+    const auto load_k = [&](int pb) {
+        const bool full = whole && pb + STEP <= p1;
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-            const int pos = pb + 16 * t + col;
-            const uint16_t* p = a.K + (size_t)min(pos, p1 - 1) * a.kd_k + g * a.hd;
+        for (int u = 0; u < LD; u++) {
+            int pos, d;
+            if (RW == 1) {  // u = t * KK + kk: position 16 t + col, 8 dims at 32 kk + 8 grp
+                pos = pb + 16 * (u / KK) + col;
+                d = 32 * (u % KK) + 8 * grp;
+            } else {
+                pos = pb + (GT * u + gt) / CH;
+                d = 8 * ((GT * u + gt) % CH);
+            }
+            if (full) {
+                kr[u] = *(const u4*)(Kg + (size_t)pos * a.kd_k + d);
+            } else {
+                const u4 z = {0, 0, 0, 0};
+                kr[u] = z;
+                if (pos < p1 && d < a.hd) kr[u] = *(const u4*)(Kg + (size_t)pos * a.kd_k + d);
+            }
+        }
+    };
+    // rows past the range are zero, as their weights are (0 * Inf is not)
+    const auto load_v = [&](int pb) {
+        const bool full = whole && pb + STEP <= p1;
+#pragma unroll
+        for (int u = 0; u < LD; u++) {
+            const int pos = pb + (GT * u + gt) / CH, d = 8 * ((GT * u + gt) % CH);
+            if (full) {
+                vr[u] = *(const u4*)(Vg + (size_t)pos * a.kd_v + d);
+            } else {
+                const u4 z = {0, 0, 0, 0};
+                vr[u] = z;
+                if (pos < p1 && d < a.hd) vr[u] = *(const u4*)(Vg + (size_t)pos * a.kd_v + d);
+            }
+        }
+    };
+    char* tile = lds + pg * S::BUFS * S::TILE;
+    const auto store_tile = [&](char* to) {
+#pragma unroll
+        for (int u = 0; u < LD; u++) {
+            const int e = GT * u + gt, rr = e / CH, ch = e % CH;
+            if (RW > 1) *(u4*)(to + rr * Lds<HD>::k_row + 16 * ch) = kr[u];
+            *(u4*)(to + (RW > 1 ? STEP * Lds<HD>::k_row : 0) + rr * Lds<HD>::v_row + 16 * ch) = vr[u];
+        }
+    };
+
+    const int steps = part / STEP;  // the same for every wave of the workgroup
+    if (steps > 0) {
+        load_v(p0);
+        load_k(p0);
+    }
+    if (RW > 1 && steps > 0) {
+        store_tile(tile);
+        __syncthreads();
+    }
+    for (int it = 0; it < steps; it++) {
+        const int pb = p0 + it * STEP;
+        const bool more = it + 1 < steps;
+        char* cur = tile + (RW > 1 ? (it & 1) * S::TILE : 0);
+        h8 kf[ST][KK];
+        if (RW == 1) {
+            if (pb >= p1) break;  // no barrier in this loop
+            store_tile(cur);
+            if (more) load_v(pb + STEP);
+#pragma unroll
+            for (int t = 0; t < ST; t++)
+#pragma unroll
+                for (int kk = 0; kk < KK; kk++) kf[t][kk] = __builtin_bit_cast(h8, kr[(t * KK + kk) % LD]);
+        } else {
+            if (more) {
+                load_k(pb + STEP);
+                load_v(pb + STEP);
+            }
+        }
+        f4 s[NQ][ST];
+#pragma unroll
+        for (int t = 0; t < ST; t++) {
+#pragma unroll
+            for (int nq = 0; nq < NQ; nq++) s[nq][t] = f4{0, 0, 0, 0};
 #pragma unroll
             for (int kk = 0; kk < KK; kk++) {
-                const int d = 32 * kk + 8 * grp;
-                u4 v = {0, 0, 0, 0};
-                if (d < a.hd && pos < p1) v = *(const u4*)(p + d);
-                kf[t][kk] = __builtin_bit_cast(h8, v);
+                const h8 k = RW == 1 ? kf[t][kk]
+                                     : *(const h8*)(cur + (16 * t + col) * Lds<HD>::k_row + 64 * kk + 16 * grp);
+#pragma unroll
+                for (int nq = 0; nq < NQ; nq++) s[nq][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[nq][kk], s[nq][t], 0, 0, 0);
+#pragma unroll
+                for (int nq = 0; nq < NQ; nq++) s[nq][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[nq][kk], s[nq][t], 0, 0, 0);
             }
         }
-        // V tile: rows past the range are zero, as their weights are (0 * Inf is not)
-#pragma unroll
-        for (int i = 0; i < kSeqTile * CH / 64; i++) {
-            const int e = 64 * i + lane, rr = e / CH, ch = e % CH;
-            const int pos = pb + rr;
-            u4 v = {0, 0, 0, 0};
-            if (8 * ch < a.hd && pos < p1) v = *(const u4*)(a.V + (size_t)pos * a.kd_v + g * a.hd + 8 * ch);
-            *(u4*)(vt + rr * HD + 8 * (ch ^ v_swizzle<HD>(rr))) = v;
-        }
-        asm volatile("" ::: "memory");
-        h8 wh[NQ], wl[NQ];
+        if (RW == 1 && more) load_k(pb + STEP);
+        h8 wh[NQ][ST / 2], wl[NQ][ST / 2];
+        const bool open = pb + STEP <= min(p1, lim_all);  // nothing in the tile is masked
 #pragma unroll
         for (int nq = 0; nq < NQ; nq++) {
-            f4 s[2];
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                s[t] = f4{0, 0, 0, 0};
-#pragma unroll
-                for (int kk = 0; kk < KK; kk++) {
-                    s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][kk], ql[nq][kk], s[t], 0, 0, 0);
-                    s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][kk], qh[nq][kk], s[t], 0, 0, 0);
-                }
-            }
             float mx = ninf;
+            if (open) {
 #pragma unroll
-            for (int t = 0; t < 2; t++)
+                for (int t = 0; t < ST; t++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int pos = pb + 16 * t + 4 * grp + j;
-                    s[t][j] = pos < min(lim[nq], p1) ? s[t][j] * c[nq] : ninf;
-                    mx = fmaxf(mx, s[t][j]);
-                }
-            if (a.scores) {
-                const int rr = rb * 16 * NQ + 16 * nq + col;
+                    for (int j = 0; j < 4; j++) mx = fmaxf(mx, s[nq][t][j]);
+            } else {
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const int pos = pb + 16 * t + 4 * grp;
-                    if (rr < rows && pos < p1)
-                        *(f4*)(a.scores + part_row[nq] * a.sstride + (pos - a.start)) = s[t];
+                for (int t = 0; t < ST; t++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (pb + 16 * t + 4 * grp + j < lim[nq]) mx = fmaxf(mx, s[nq][t][j]);
+            }
+            if (!OWN && a.scores) {
+                const int rr = row0 + 16 * nq + col;
+                if (rr < rows) {
+                    const int i = rr / a.r;
+                    float* to = a.scores + ((size_t)i * a.n_heads + g * a.r + (rr - i * a.r)) * a.sstride - a.start;
+#pragma unroll
+                    for (int t = 0; t < ST; t++) {
+                        const int pos = pb + 16 * t + 4 * grp;
+                        f4 x;
+#pragma unroll
+                        for (int j = 0; j < 4; j++) x[j] = pos + j < lim[nq] ? s[nq][t][j] * c[nq] : ninf;
+                        if (pos < p1) *(f4*)(to + pos) = x;
+                    }
                 }
             }
             mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const float nb = fmaxf(base[nq], mx - kSeqLift);
+            const float nb = mx == ninf ? base[nq] : fmaxf(base[nq], mx * c[nq] - kSeqLift);
             if (__any(nb > base[nq])) {
-                const float f = base[nq] == ninf ? 0.0f : __builtin_amdgcn_exp2f(base[nq] - nb);
+                const float f = nb == base[nq] ? 1.0f : __builtin_amdgcn_exp2f(base[nq] - nb);
                 l[nq] *= f;
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++) o[nq][dt] *= f;
                 base[nq] = nb;
             }
-            const float bs = nb == ninf ? 0.0f : nb;  // nothing so far: every weight is 0
+            f4 w[ST];
 #pragma unroll
-            for (int t = 0; t < 2; t++)
+            for (int t = 0; t < ST; t++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const float w = __builtin_amdgcn_exp2f(s[t][j] - bs);
-                    l[nq] += w;
-                    const _Float16 hi = (_Float16)w;
-                    wh[nq][4 * t + j] = hi;
-                    wl[nq][4 * t + j] = (_Float16)(w - (float)hi);
+                for (int j = 0; j < 4; j++) w[t][j] = __builtin_amdgcn_exp2f(fmaf(s[nq][t][j], c[nq], -nb));
+            if (!open) {
+#pragma unroll
+                for (int t = 0; t < ST; t++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (!(pb + 16 * t + 4 * grp + j < lim[nq])) w[t][j] = 0.0f;
+            }
+            // the two parts of a weight, both cut short: 21 bits
+#pragma unroll
+            for (int t = 0; t < ST; t++)
+#pragma unroll
+                for (int j = 0; j < 4; j += 2) {
+                    l[nq] += w[t][j] + w[t][j + 1];
+                    const auto hi = __builtin_amdgcn_cvt_pkrtz(w[t][j], w[t][j + 1]);
+                    const auto lo = __builtin_amdgcn_cvt_pkrtz(fmaf(-1.0f, (float)hi[0], w[t][j]), fmaf(-1.0f, (float)hi[1], w[t][j + 1]));
+                    const int at = 4 * (t & 1) + j;
+                    wh[nq][t / 2][at] = (_Float16)hi[0];
+                    wh[nq][t / 2][at + 1] = (_Float16)hi[1];
+                    wl[nq][t / 2][at] = (_Float16)lo[0];
+                    wl[nq][t / 2][at + 1] = (_Float16)lo[1];
                 }
         }
-        // operand k = 8 grp + 4 t + j is position 16 t + 4 grp + j
+        // operand k = 8 grp + 4 t + j of step u is position 32 u + 16 t + 4 grp + j
+        const char* vt = cur + (RW > 1 ? STEP * Lds<HD>::k_row : 0) + (4 * grp + (col >> 2)) * Lds<HD>::v_row + 8 * (col & 3);
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++) {
-            h8 vf;
+        for (int u = 0; u < ST / 2; u++)
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const int rr = 16 * t + 4 * grp + (col >> 2), d = 16 * dt + 4 * (col & 3);
-                s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) s4*)(vt + rr * HD + 8 * ((d >> 3) ^ v_swizzle<HD>(rr)) + (d & 7)));
-                const h4 y = __builtin_bit_cast(h4, x);
+            for (int dt = 0; dt < DT; dt++) {
+                s4 x[2];
 #pragma unroll
-                for (int j = 0; j < 4; j++) vf[4 * t + j] = y[j];
+                for (int t = 0; t < 2; t++)
+                    x[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) s4*)(vt + (32 * u + 16 * t) * Lds<HD>::v_row + 32 * dt));
+                const h8 vf = join(x[0], x[1]);
+#pragma unroll
+                for (int nq = 0; nq < NQ; nq++) o[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, wl[nq][u], o[nq][dt], 0, 0, 0);
+#pragma unroll
+                for (int nq = 0; nq < NQ; nq++) o[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, wh[nq][u], o[nq][dt], 0, 0, 0);
             }
-#pragma unroll
-            for (int nq = 0; nq < NQ; nq++) {
-                o[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, wl[nq], o[nq][dt], 0, 0, 0);
-                o[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, wh[nq], o[nq][dt], 0, 0, 0);
-            }
-        }
         asm volatile("" ::: "memory");
+        if (RW > 1) {
+            if (more) store_tile(tile + ((it + 1) & 1) * S::TILE);
+            __syncthreads();
+        }
     }
-    // the waves' results: one tile of query rows at a time through LDS
+
+    // results: straight to the partials, or the position groups' joined in LDS,
+    // one tile of query rows of every row wave at a time
 #pragma unroll
     for (int nq = 0; nq < NQ; nq++) {
         float ls = l[nq];
         ls += __shfl_xor(ls, 16);
         ls += __shfl_xor(ls, 32);
+        if (PW == 1) {
+            const int rr = row0 + 16 * nq + col;
+            if (rr < rows) {
+                const int i = OWN ? tok : rr / a.r, hh = OWN ? rr : rr - i * a.r;
+                const size_t at = ((size_t)i * a.n_heads + g * a.r + hh) * a.slots + slot + (OWN ? a.slot0 : 0);
+                if (grp == 0) {
+                    a.pm[at] = base[nq];
+                    a.pl[at] = ls;
+                }
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++)
+                    if (16 * dt + 4 * grp < a.hd) *(f4*)(a.po + at * a.hd + 16 * dt + 4 * grp) = o[nq][dt];
+            }
+            continue;
+        }
+        float* so = (float*)lds;  // [wave][16][HD + 4]
         __syncthreads();
         if (grp == 0) {
             sm[wave][col] = base[nq];
             sl[wave][col] = ls;
         }
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++) *(f4*)&so[wave][col][16 * dt + 4 * grp] = o[nq][dt];
+        for (int dt = 0; dt < DT; dt++) *(f4*)(so + (wave * 16 + col) * (HD + 4) + 16 * dt + 4 * grp) = o[nq][dt];
         __syncthreads();
-        // thread t: row t / 16, dims (t % 16) * 4 + 64 u
-        const int row = threadIdx.x >> 4, rr = rb * 16 * NQ + 16 * nq + row;
-        float M = ninf, L = 0.0f, f[kSeqWaves];
+        // 16 threads a row: RW * 16 rows, dims 4 (t % 16) + 64 v
 #pragma unroll
-        for (int w = 0; w < kSeqWaves; w++) M = fmaxf(M, sm[w][row]);
+        for (int q = 0; q < RW; q++) {
+            const int row = threadIdx.x >> 4, rr = (rb * RW + q) * 16 * NQ + 16 * nq + row;
+            float M = ninf, L = 0.0f, f[PW];
 #pragma unroll
-        for (int w = 0; w < kSeqWaves; w++) {
-            f[w] = sm[w][row] == ninf ? 0.0f : __builtin_amdgcn_exp2f(sm[w][row] - M);
-            L = fmaf(sl[w][row], f[w], L);
-        }
-        if (rr < rows) {
-            const int i = OWN ? tok : rr / a.r, hh = OWN ? rr : rr - i * a.r;
-            const size_t at = ((size_t)i * a.n_heads + g * a.r + hh) * a.slots + a.slot0 + slot;
-            if ((threadIdx.x & 15) == 0) {
-                a.pm[at] = M;
-                a.pl[at] = L;
+            for (int w = 0; w < PW; w++) M = fmaxf(M, sm[w * RW + q][row]);
+#pragma unroll
+            for (int w = 0; w < PW; w++) {
+                const float m = sm[w * RW + q][row];
+                f[w] = m == ninf ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+                L = fmaf(sl[w * RW + q][row], f[w], L);
             }
-            for (int d = 4 * (threadIdx.x & 15); d < a.hd; d += 64) {
-                f4 x = {0, 0, 0, 0};
+            if (rr < rows) {
+                const int i = OWN ? tok : rr / a.r, hh = OWN ? rr : rr - i * a.r;
+                const size_t at = ((size_t)i * a.n_heads + g * a.r + hh) * a.slots + slot + (OWN ? a.slot0 : 0);
+                if ((threadIdx.x & 15) == 0) {
+                    a.pm[at] = M;
+                    a.pl[at] = L;
+                }
+                for (int d = 4 * (threadIdx.x & 15); d < a.hd; d += 64) {
+                    f4 x = {0, 0, 0, 0};
 #pragma unroll
-                for (int w = 0; w < kSeqWaves; w++) x += f[w] * *(const f4*)&so[w][row][d];
-                *(f4*)(a.po + at * a.hd + d) = x;
+                    for (int w = 0; w < PW; w++) x += f[w] * *(const f4*)(so + ((w * RW + q) * 16 + row) * (HD + 4) + d);
+                    *(f4*)(a.po + at * a.hd + d) = x;
+                }
             }
         }
     }
 }
 
+// Shared and own ranges in one launch: own_wgs workgroups of own ranges among
+// the shared ones.
+template <int HD, int NQ, int RW>
+__global__ __launch_bounds__(256) void seq_attend_kernel(SeqArgs a) {
+    constexpr int A = SeqShape<HD, NQ, RW>::BYTES, B = SeqShape<HD, 1, 1>::BYTES;
+    __shared__ __align__(16) char lds[A > B ? A : B];
+    __shared__ float sm[kSeqWaves][16], sl[kSeqWaves][16];
+    const int b = blockIdx.x;
+    if (b < a.shared_wgs) seq_run<HD, NQ, RW, false>(a, b, lds, sm, sl);
+    else seq_run<HD, 1, 1, true>(a, b - a.shared_wgs, lds, sm, sl);
+}
+
 // out[row] = sum_s 2^(base_s - M) o_s / sum_s 2^(base_s - M) l_s; a row
-// without positions is zero.  ml, if set: M and 1 / sum of each row.
-__global__ __launch_bounds__(128) void seq_merge_kernel(const float* __restrict__ pm, const float* __restrict__ pl,
-                                                        const float* __restrict__ po, int slots, int hd,
+// without positions is zero.  ml, if set: M and 1 / sum of each row.  One wave
+// a row: lane s holds slot s's factor (at most 2 * kSeqMaxSplits slots), then
+// the lanes take the dims, eight slots' loads in flight.
+__global__ __launch_bounds__(256) void seq_merge_kernel(const float* __restrict__ pm, const float* __restrict__ pl,
+                                                        const float* __restrict__ po, int rows, int slots, int hd,
                                                         float* __restrict__ out, float* __restrict__ ml) {
-    const size_t row = blockIdx.x;
-    const int d = threadIdx.x;
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (row >= rows) return;
     const float ninf = -__int_as_float(0x7f800000);
-    pm += row * slots;
-    pl += row * slots;
-    float M = ninf;
-    for (int s = 0; s < slots; s++) M = fmaxf(M, pm[s]);
-    float L = 0.0f, o = 0.0f;
-    for (int s = 0; s < slots; s++) {
-        const float f = pm[s] == ninf ? 0.0f : __builtin_amdgcn_exp2f(pm[s] - M);
-        L = fmaf(pl[s], f, L);
-        if (d < hd) o = fmaf(po[(row * slots + s) * hd + d], f, o);
-    }
+    const size_t at = (size_t)row * slots;
+    static_assert(2 * kSeqMaxSplits == 128, "two slots a lane");
+    const float m0 = lane < slots ? pm[at + lane] : ninf, m1 = lane + 64 < slots ? pm[at + lane + 64] : ninf;
+    const float l0 = lane < slots ? pl[at + lane] : 0.0f, l1 = lane + 64 < slots ? pl[at + lane + 64] : 0.0f;
+    const float M = wave_max(fmaxf(m0, m1));
+    const float f0 = m0 == ninf ? 0.0f : __builtin_amdgcn_exp2f(m0 - M), f1 = m1 == ninf ? 0.0f : __builtin_amdgcn_exp2f(m1 - M);
+    float L = fmaf(l0, f0, l1 * f1);
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) L += __shfl_xor(L, off);
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    if (d < hd) out[row * hd + d] = L == 0.0f ? 0.0f : o * inv;
-    if (ml && d == 0) {
-        ml[2 * row] = M;
-        ml[2 * row + 1] = inv;
+    if (ml && lane == 0) {
+        ml[2 * (size_t)row] = M;
+        ml[2 * (size_t)row + 1] = inv;
     }
+    const int d = 2 * lane;
+    float o0 = 0.0f, o1 = 0.0f;
+    const float* p = po + at * hd + (d < hd ? d : 0);
+#pragma unroll 8
+    for (int s = 0; s < slots; s++) {
+        const float f = readlane_f(s < 64 ? f0 : f1, s & 63);
+        const float2 x = *(const float2*)(p + (size_t)s * hd);
+        o0 = fmaf(x.x, f, o0);
+        o1 = fmaf(x.y, f, o1);
+    }
+    if (d < hd) *(float2*)(out + (size_t)row * hd + d) = make_float2(L == 0.0f ? 0.0f : o0 * inv, L == 0.0f ? 0.0f : o1 * inv);
 }
 
 // mass[g][start + t] += the weights of position t over the rows of kv head g
@@ -344,17 +501,12 @@ __global__ __launch_bounds__(256) void seq_mass_kernel(const float* __restrict__
     mass[(size_t)g * mass_stride + t] += sum;
 }
 
-template <int HD, int NQ, bool OWN>
-static void seq_launch(const SeqArgs& a, int blocks, hipStream_t s) {
-    hipLaunchKernelGGL((seq_attend_kernel<HD, NQ, OWN>), dim3(blocks), dim3(256), 0, s, a);
-}
-
-template <int NQ, bool OWN>
+template <int NQ, int RW>
 static void seq_launch_hd(const SeqArgs& a, int blocks, hipStream_t s) {
-    if (a.hd <= 32) seq_launch<32, NQ, OWN>(a, blocks, s);
-    else if (a.hd <= 64) seq_launch<64, NQ, OWN>(a, blocks, s);
-    else if (a.hd <= 96) seq_launch<96, NQ, OWN>(a, blocks, s);
-    else seq_launch<128, NQ, OWN>(a, blocks, s);
+    if (a.hd <= 32) hipLaunchKernelGGL((seq_attend_kernel<32, NQ, RW>), dim3(blocks), dim3(256), 0, s, a);
+    else if (a.hd <= 64) hipLaunchKernelGGL((seq_attend_kernel<64, NQ, RW>), dim3(blocks), dim3(256), 0, s, a);
+    else if (a.hd <= 96) hipLaunchKernelGGL((seq_attend_kernel<96, NQ, RW>), dim3(blocks), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((seq_attend_kernel<128, NQ, RW>), dim3(blocks), dim3(256), 0, s, a);
 }
 
 static int seq_check(const char* what, const gllm_hip_kv* kv, int l, const float* d_q, int n, int n_heads, int n_kv,
@@ -415,11 +567,17 @@ static SeqArgs seq_args(const gllm_hip_kv* kv, int l, const float* d_q, int n, i
     return a;
 }
 
-static void seq_shared(const SeqArgs& a, const SeqPlan& p, hipStream_t s) {
-    const int blocks = a.n_kv * p.row_blocks * p.chunks;
-    if (p.nq == 1) seq_launch_hd<1, false>(a, blocks, s);
-    else if (p.nq == 2) seq_launch_hd<2, false>(a, blocks, s);
-    else seq_launch_hd<4, false>(a, blocks, s);
+static int seq_launch(SeqArgs a, const SeqPlan& p, hipStream_t s) {
+    a.shared_wgs = a.n_kv * p.row_blocks * p.chunks;
+    a.slot0 = p.chunks;
+    const long long blocks = a.shared_wgs + (long long)a.n_kv * p.own_blocks * a.n * p.splits;
+    if (blocks == 0) return GLLM_OK;
+    if (p.nq == 1) seq_launch_hd<1, 1>(a, (int)blocks, s);
+    else if (p.rw == 1) seq_launch_hd<2, 1>(a, (int)blocks, s);
+    else if (p.rw == 2) seq_launch_hd<2, 2>(a, (int)blocks, s);
+    else seq_launch_hd<2, 4>(a, (int)blocks, s);
+    GLLM_HIP(hipGetLastError());
+    return GLLM_OK;
 }
 
 }  // namespace gllm
@@ -453,16 +611,8 @@ int gllm_hip_attend_shared_dev(gllm_hip_kv* kv, int l, const float* d_q, int n, 
     a.len = len;
     a.starts = d_starts;
     a.lens = d_lens;
-    if (p.chunks) {
-        seq_shared(a, p, s);
-        GLLM_HIP(hipGetLastError());
-    }
-    if (p.splits) {
-        a.slot0 = p.chunks;
-        seq_launch_hd<1, true>(a, n_kv_heads * p.own_blocks * n * p.splits, s);
-        GLLM_HIP(hipGetLastError());
-    }
-    hipLaunchKernelGGL(seq_merge_kernel, dim3((unsigned)p.rows), dim3(128), 0, s, a.pm, a.pl, a.po, p.slots, hd, d_out,
+    GLLM_TRY(seq_launch(a, p, s));
+    hipLaunchKernelGGL(seq_merge_kernel, dim3((unsigned)((p.rows + 3) / 4)), dim3(256), 0, s, a.pm, a.pl, a.po, (int)p.rows, p.slots, hd, d_out,
                        (float*)nullptr);
     GLLM_HIP(hipGetLastError());
     return GLLM_OK;
@@ -496,9 +646,8 @@ int gllm_hip_attend_mass_dev(gllm_hip_kv* kv, int l, const float* d_q, int n, in
     a.causal = 1;
     a.scores = w;
     a.sstride = sstride;
-    seq_shared(a, p, s);
-    GLLM_HIP(hipGetLastError());
-    hipLaunchKernelGGL(seq_merge_kernel, dim3((unsigned)p.rows), dim3(128), 0, s, a.pm, a.pl, a.po, p.slots, hd, d_out, ml);
+    GLLM_TRY(seq_launch(a, p, s));
+    hipLaunchKernelGGL(seq_merge_kernel, dim3((unsigned)((p.rows + 3) / 4)), dim3(256), 0, s, a.pm, a.pl, a.po, (int)p.rows, p.slots, hd, d_out, ml);
     GLLM_HIP(hipGetLastError());
     hipLaunchKernelGGL(seq_mass_kernel, dim3((len + 255) / 256, n_kv_heads), dim3(256), 0, s, w, sstride, ml, n, n_heads,
                        p.r, len, d_mass + start, mass_stride);

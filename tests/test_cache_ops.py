@@ -32,7 +32,7 @@ int main() {
         const SeqPlan p = seq_plan(n, h, g, len, most);
         plans++;
         need(p.r == r && p.rows == (size_t)n * h, "rows", n, h, g, len, most);
-        need((long long)p.row_blocks * 16 * p.nq >= (long long)n * r, "row blocks", n, h, g, len, most);
+        need((long long)p.row_blocks * 16 * p.nq * p.rw >= (long long)n * r, "row blocks", n, h, g, len, most);
         need(p.chunks <= kSeqMaxSplits && p.splits <= kSeqMaxSplits && p.slots == p.chunks + p.splits, "slots", n, h, g, len, most);
         need((len > 0) == (p.chunks > 0) && (most > 0) == (p.splits > 0), "parts", n, h, g, len, most);
         if (len) {
