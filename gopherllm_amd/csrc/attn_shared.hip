@@ -58,6 +58,7 @@ struct SeqArgs {
 };
 
 constexpr float kSeqLift = 15.0f;
+constexpr int kBufferWord3 = 0x00020000;  // raw buffer of 32-bit data; reads past its end give 0
 
 // Bytes between rows of an LDS tile.  K rows are read 16 bytes a lane, eight
 // rows at a time: 16 bytes of padding spread them over the banks.  V rows are
@@ -101,7 +102,7 @@ __device__ __forceinline__ void seq_run(const SeqArgs& a, int b, char* lds, floa
     constexpr int GT = RW * 64;                    // threads of a position group
     constexpr int LD = STEP * CH / GT;             // 16-byte loads of a thread for a tile
     static_assert(STEP * CH % GT == 0, "a tile is a whole number of loads");
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
     const int pg = wave / RW, rw = wave % RW;
     const float ninf = -__int_as_float(0x7f800000);
@@ -184,48 +185,36 @@ __device__ __forceinline__ void seq_run(const SeqArgs& a, int b, char* lds, floa
         for (int dt = 0; dt < DT; dt++) o[nq][dt] = f4{0, 0, 0, 0};
     }
 
-    // a tile's K and V as loads: RW > 1: chunk e = GT u + thread of the group,
-    // to LDS; RW == 1: K straight into operand order
-    const uint16_t* Kg = a.K + g * a.hd;
-    const uint16_t* Vg = a.V + g * a.hd;
-    const bool whole = a.hd == HD;
+    // A tile's K and V as loads.  V, and K where waves share it, go to LDS: 16-byte
+    // chunk e = GT u + thread of the group; K of a wave's own goes straight into
+    // operand order, u = t * KK + kk: position 16 t + col, dims 32 kk + 8 grp.
+    // The buffer ends with the range's last row, so what is past it reads as
+    // zero without a branch (V has to: the weight there is 0, and 0 * Inf is not);
+    // dims past hd get an offset past any buffer.
     const int gt = rw * 64 + lane;
     u4 kr[LD], vr[LD];
+    const auto rsrc = [&](const uint16_t* base, int kd, int pb) {
+        const int n = min(p1 - pb, STEP);
+        return __builtin_amdgcn_make_buffer_rsrc((void*)(base + (size_t)pb * kd + g * a.hd), 0,
+                                                 n > 0 ? ((n - 1) * kd + a.hd) * 2 : 0, kBufferWord3);
+    };
+    const auto chunk_off = [&](int u, int kd) {
+        const int e = GT * u + gt, d = 8 * (e % CH);
+        return d < a.hd ? (e / CH * kd + d) * 2 : (int)0x80000000;
+    };
     const auto load_k = [&](int pb) {
-        const bool full = whole && pb + STEP <= p1;
+        const auto r = rsrc(a.K, a.kd_k, pb);
 #pragma unroll
         for (int u = 0; u < LD; u++) {
-            int pos, d;
-            if (RW == 1) {  // u = t * KK + kk: position 16 t + col, 8 dims at 32 kk + 8 grp
-                pos = pb + 16 * (u / KK) + col;
-                d = 32 * (u % KK) + 8 * grp;
-            } else {
-                pos = pb + (GT * u + gt) / CH;
-                d = 8 * ((GT * u + gt) % CH);
-            }
-            if (full) {
-                kr[u] = *(const u4*)(Kg + (size_t)pos * a.kd_k + d);
-            } else {
-                const u4 z = {0, 0, 0, 0};
-                kr[u] = z;
-                if (pos < p1 && d < a.hd) kr[u] = *(const u4*)(Kg + (size_t)pos * a.kd_k + d);
-            }
+            const int t = u / KK, d = 32 * (u % KK) + 8 * grp;
+            const int off = RW > 1 ? chunk_off(u, a.kd_k) : d < a.hd ? ((16 * t + col) * a.kd_k + d) * 2 : (int)0x80000000;
+            kr[u] = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
         }
     };
-    // rows past the range are zero, as their weights are (0 * Inf is not)
     const auto load_v = [&](int pb) {
-        const bool full = whole && pb + STEP <= p1;
+        const auto r = rsrc(a.V, a.kd_v, pb);
 #pragma unroll
-        for (int u = 0; u < LD; u++) {
-            const int pos = pb + (GT * u + gt) / CH, d = 8 * ((GT * u + gt) % CH);
-            if (full) {
-                vr[u] = *(const u4*)(Vg + (size_t)pos * a.kd_v + d);
-            } else {
-                const u4 z = {0, 0, 0, 0};
-                vr[u] = z;
-                if (pos < p1 && d < a.hd) vr[u] = *(const u4*)(Vg + (size_t)pos * a.kd_v + d);
-            }
-        }
+        for (int u = 0; u < LD; u++) vr[u] = __builtin_amdgcn_raw_buffer_load_b128(r, chunk_off(u, a.kd_v), 0, 0);
     };
     char* tile = lds + pg * S::BUFS * S::TILE;
     const auto store_tile = [&](char* to) {
@@ -237,6 +226,8 @@ __device__ __forceinline__ void seq_run(const SeqArgs& a, int b, char* lds, floa
         }
     };
 
+    float minus1 = -1.0f;  // a register, so that w - hi is one mixed-precision fma of hi as it lies
+    asm volatile("" : "+v"(minus1));
     const int steps = part / STEP;  // the same for every wave of the workgroup
     if (steps > 0) {
         load_v(p0);
@@ -342,7 +333,7 @@ __device__ __forceinline__ void seq_run(const SeqArgs& a, int b, char* lds, floa
                 for (int j = 0; j < 4; j += 2) {
                     l[nq] += w[t][j] + w[t][j + 1];
                     const auto hi = __builtin_amdgcn_cvt_pkrtz(w[t][j], w[t][j + 1]);
-                    const auto lo = __builtin_amdgcn_cvt_pkrtz(fmaf(-1.0f, (float)hi[0], w[t][j]), fmaf(-1.0f, (float)hi[1], w[t][j + 1]));
+                    const auto lo = __builtin_amdgcn_cvt_pkrtz(fmaf((float)hi[0], minus1, w[t][j]), fmaf((float)hi[1], minus1, w[t][j + 1]));
                     const int at = 4 * (t & 1) + j;
                     wh[nq][t / 2][at] = (_Float16)hi[0];
                     wh[nq][t / 2][at + 1] = (_Float16)hi[1];
@@ -439,7 +430,7 @@ __device__ __forceinline__ void seq_run(const SeqArgs& a, int b, char* lds, floa
 // Shared and own ranges in one launch: own_wgs workgroups of own ranges among
 // the shared ones.
 template <int HD, int NQ, int RW>
-__global__ __launch_bounds__(256) void seq_attend_kernel(SeqArgs a) {
+__global__ __launch_bounds__(256, 2) void seq_attend_kernel(SeqArgs a) {
     constexpr int A = SeqShape<HD, NQ, RW>::BYTES, B = SeqShape<HD, 1, 1>::BYTES;
     __shared__ __align__(16) char lds[A > B ? A : B];
     __shared__ float sm[kSeqWaves][16], sl[kSeqWaves][16];
@@ -572,8 +563,8 @@ static int seq_launch(SeqArgs a, const SeqPlan& p, hipStream_t s) {
     a.slot0 = p.chunks;
     const long long blocks = a.shared_wgs + (long long)a.n_kv * p.own_blocks * a.n * p.splits;
     if (blocks == 0) return GLLM_OK;
-    if (p.nq == 1) seq_launch_hd<1, 1>(a, (int)blocks, s);
-    else if (p.rw == 1) seq_launch_hd<2, 1>(a, (int)blocks, s);
+    if (p.rw == 1) seq_launch_hd<1, 1>(a, (int)blocks, s);
+    else if (p.nq == 1) seq_launch_hd<1, 2>(a, (int)blocks, s);
     else if (p.rw == 2) seq_launch_hd<2, 2>(a, (int)blocks, s);
     else seq_launch_hd<2, 4>(a, (int)blocks, s);
     GLLM_HIP(hipGetLastError());
