@@ -57,8 +57,7 @@ inline SeqPlan seq_plan(int n, int n_heads, int n_kv, int len, int most) {
 inline size_t seq_floats(const SeqPlan& p, int hd, size_t scored) {
     const size_t parts = p.rows * (size_t)p.slots;
     size_t f = parts * (2 + (size_t)hd);
-    if (scored) f += p.rows * (scored + 2);
-    return f + 64;
+    return f + p.rows * scored + 64;
 }
 
 // Rows a .. b - 1 of a cache of max_len rows that the range start, len names.

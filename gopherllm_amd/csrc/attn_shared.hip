@@ -128,6 +128,43 @@ __device__ __forceinline__ void seq_run(const SeqArgs& a, int b, char* lds, floa
     const int part = ((a1 - a0 + PW * STEP - 1) / (PW * STEP)) * STEP;  // positions of a group
     const int p0 = min(a1, a0 + pg * part), p1 = min(a1, p0 + part);
 
+    // A tile's K and V as loads.  V, and K where waves share it, go to LDS: 16-byte
+    // chunk e = GT u + thread of the group; K of a wave's own goes straight into
+    // operand order, u = t * KK + kk: position 16 t + col, dims 32 kk + 8 grp.
+    // The buffer ends with the range's last row, so what is past it reads as
+    // zero without a branch (V has to: the weight there is 0, and 0 * Inf is not);
+    // dims past hd get an offset past any buffer.
+    const int gt = rw * 64 + lane;
+    u4 kr[LD], vr[LD];
+    const auto rsrc = [&](const uint16_t* base, int kd, int pb) {
+        const int n = min(p1 - pb, STEP);
+        return __builtin_amdgcn_make_buffer_rsrc((void*)(base + (size_t)pb * kd + g * a.hd), 0,
+                                                 n > 0 ? ((n - 1) * kd + a.hd) * 2 : 0, kBufferWord3);
+    };
+    const auto chunk_off = [&](int u, int kd) {
+        const int e = GT * u + gt, d = 8 * (e % CH);
+        return d < a.hd ? (e / CH * kd + d) * 2 : (int)0x80000000;
+    };
+    const auto load_k = [&](int pb) {
+        const auto r = rsrc(a.K, a.kd_k, pb);
+#pragma unroll
+        for (int u = 0; u < LD; u++) {
+            const int t = u / KK, d = 32 * (u % KK) + 8 * grp;
+            const int off = RW > 1 ? chunk_off(u, a.kd_k) : d < a.hd ? ((16 * t + col) * a.kd_k + d) * 2 : (int)0x80000000;
+            kr[u] = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
+        }
+    };
+    const auto load_v = [&](int pb) {
+        const auto r = rsrc(a.V, a.kd_v, pb);
+#pragma unroll
+        for (int u = 0; u < LD; u++) vr[u] = __builtin_amdgcn_raw_buffer_load_b128(r, chunk_off(u, a.kd_v), 0, 0);
+    };
+    const int steps = part / STEP;  // the same for every wave of the workgroup
+    if (steps > 0) {  // on their way while the query rows are read and split
+        load_v(p0);
+        load_k(p0);
+    }
+
     // query rows: rb * 16 * NQ * RW + 16 * (rw * NQ + nq) + col of this kv head
     const int rows = OWN ? a.r : a.n * a.r;
     const int row0 = (rb * RW + rw) * 16 * NQ;
@@ -185,37 +222,6 @@ __device__ __forceinline__ void seq_run(const SeqArgs& a, int b, char* lds, floa
         for (int dt = 0; dt < DT; dt++) o[nq][dt] = f4{0, 0, 0, 0};
     }
 
-    // A tile's K and V as loads.  V, and K where waves share it, go to LDS: 16-byte
-    // chunk e = GT u + thread of the group; K of a wave's own goes straight into
-    // operand order, u = t * KK + kk: position 16 t + col, dims 32 kk + 8 grp.
-    // The buffer ends with the range's last row, so what is past it reads as
-    // zero without a branch (V has to: the weight there is 0, and 0 * Inf is not);
-    // dims past hd get an offset past any buffer.
-    const int gt = rw * 64 + lane;
-    u4 kr[LD], vr[LD];
-    const auto rsrc = [&](const uint16_t* base, int kd, int pb) {
-        const int n = min(p1 - pb, STEP);
-        return __builtin_amdgcn_make_buffer_rsrc((void*)(base + (size_t)pb * kd + g * a.hd), 0,
-                                                 n > 0 ? ((n - 1) * kd + a.hd) * 2 : 0, kBufferWord3);
-    };
-    const auto chunk_off = [&](int u, int kd) {
-        const int e = GT * u + gt, d = 8 * (e % CH);
-        return d < a.hd ? (e / CH * kd + d) * 2 : (int)0x80000000;
-    };
-    const auto load_k = [&](int pb) {
-        const auto r = rsrc(a.K, a.kd_k, pb);
-#pragma unroll
-        for (int u = 0; u < LD; u++) {
-            const int t = u / KK, d = 32 * (u % KK) + 8 * grp;
-            const int off = RW > 1 ? chunk_off(u, a.kd_k) : d < a.hd ? ((16 * t + col) * a.kd_k + d) * 2 : (int)0x80000000;
-            kr[u] = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
-        }
-    };
-    const auto load_v = [&](int pb) {
-        const auto r = rsrc(a.V, a.kd_v, pb);
-#pragma unroll
-        for (int u = 0; u < LD; u++) vr[u] = __builtin_amdgcn_raw_buffer_load_b128(r, chunk_off(u, a.kd_v), 0, 0);
-    };
     char* tile = lds + pg * S::BUFS * S::TILE;
     const auto store_tile = [&](char* to) {
 #pragma unroll
@@ -228,11 +234,6 @@ __device__ __forceinline__ void seq_run(const SeqArgs& a, int b, char* lds, floa
 
     float minus1 = -1.0f;  // a register, so that w - hi is one mixed-precision fma of hi as it lies
     asm volatile("" : "+v"(minus1));
-    const int steps = part / STEP;  // the same for every wave of the workgroup
-    if (steps > 0) {
-        load_v(p0);
-        load_k(p0);
-    }
     if (RW > 1 && steps > 0) {
         store_tile(tile);
         __syncthreads();
@@ -439,57 +440,98 @@ __global__ __launch_bounds__(256, 2) void seq_attend_kernel(SeqArgs a) {
     else seq_run<HD, 1, 1, true>(a, b - a.shared_wgs, lds, sm, sl);
 }
 
-// out[row] = sum_s 2^(base_s - M) o_s / sum_s 2^(base_s - M) l_s; a row
-// without positions is zero.  ml, if set: M and 1 / sum of each row.  One wave
-// a row: lane s holds slot s's factor (at most 2 * kSeqMaxSplits slots), then
-// the lanes take the dims, eight slots' loads in flight.
-__global__ __launch_bounds__(256) void seq_merge_kernel(const float* __restrict__ pm, const float* __restrict__ pl,
-                                                        const float* __restrict__ po, int rows, int slots, int hd,
-                                                        float* __restrict__ out, float* __restrict__ ml) {
-    const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (row >= rows) return;
-    const float ninf = -__int_as_float(0x7f800000);
-    const size_t at = (size_t)row * slots;
+// The factor of each of a row's slots (two a lane), and the row's base and sum.
+struct SlotFactors {
+    float f0, f1, M, L;
+};
+__device__ __forceinline__ SlotFactors slot_factors(const float* pm, const float* pl, size_t at, int slots, int lane) {
     static_assert(2 * kSeqMaxSplits == 128, "two slots a lane");
+    const float ninf = -__int_as_float(0x7f800000);
     const float m0 = lane < slots ? pm[at + lane] : ninf, m1 = lane + 64 < slots ? pm[at + lane + 64] : ninf;
     const float l0 = lane < slots ? pl[at + lane] : 0.0f, l1 = lane + 64 < slots ? pl[at + lane + 64] : 0.0f;
-    const float M = wave_max(fmaxf(m0, m1));
-    const float f0 = m0 == ninf ? 0.0f : __builtin_amdgcn_exp2f(m0 - M), f1 = m1 == ninf ? 0.0f : __builtin_amdgcn_exp2f(m1 - M);
-    float L = fmaf(l0, f0, l1 * f1);
+    SlotFactors r;
+    r.M = wave_max(fmaxf(m0, m1));
+    r.f0 = m0 == ninf ? 0.0f : __builtin_amdgcn_exp2f(m0 - r.M);
+    r.f1 = m1 == ninf ? 0.0f : __builtin_amdgcn_exp2f(m1 - r.M);
+    r.L = fmaf(l0, r.f0, l1 * r.f1);
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) L += __shfl_xor(L, off);
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    if (ml && lane == 0) {
-        ml[2 * (size_t)row] = M;
-        ml[2 * (size_t)row + 1] = inv;
-    }
-    const int d = 2 * lane;
-    float o0 = 0.0f, o1 = 0.0f;
-    const float* p = po + at * hd + (d < hd ? d : 0);
-#pragma unroll 8
-    for (int s = 0; s < slots; s++) {
-        const float f = readlane_f(s < 64 ? f0 : f1, s & 63);
-        const float2 x = *(const float2*)(p + (size_t)s * hd);
-        o0 = fmaf(x.x, f, o0);
-        o1 = fmaf(x.y, f, o1);
-    }
-    if (d < hd) *(float2*)(out + (size_t)row * hd + d) = make_float2(L == 0.0f ? 0.0f : o0 * inv, L == 0.0f ? 0.0f : o1 * inv);
+    for (int off = 32; off >= 1; off >>= 1) r.L += __shfl_xor(r.L, off);
+    return r;
 }
 
-// mass[g][start + t] += the weights of position t over the rows of kv head g
-__global__ __launch_bounds__(256) void seq_mass_kernel(const float* __restrict__ scores, int sstride,
-                                                       const float* __restrict__ ml, int n, int n_heads, int r,
-                                                       int len, float* __restrict__ mass, int mass_stride) {
-    const int g = blockIdx.y, t = blockIdx.x * 256 + threadIdx.x;
-    if (t >= len) return;
-    float sum = 0.0f;
-    for (int i = 0; i < n; i++)
-        for (int h = 0; h < r; h++) {
-            const size_t row = (size_t)i * n_heads + g * r + h;
-            const float inv = ml[2 * row + 1];
-            if (inv != 0.0f) sum += __builtin_amdgcn_exp2f(scores[row * sstride + t] - ml[2 * row]) * inv;
+struct MergeArgs {
+    const float *pm, *pl, *po;
+    float* out;
+    int rows, slots, hd;
+    const float* scores;  // [row][sstride], or null: no mass
+    float* mass;          // [kv head][mass_stride], from the first attended row on
+    int sstride, n, n_heads, n_kv, r, len, mass_stride, mass_wgs;
+};
+
+constexpr int kMassRows = 64;  // query rows whose base and 1 / sum a workgroup holds at a time
+
+// Workgroups below mass_wgs add the weights of 512 positions to mass, the
+// others make a row's output:
+// out[row] = sum_s 2^(base_s - M) o_s / sum_s 2^(base_s - M) l_s, zero for a row
+// without positions; 32 threads take a slot, 4 dims each, eight slots at a time.
+__global__ __launch_bounds__(256) void seq_merge_kernel(MergeArgs a) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ __align__(16) float red[8][128];
+    if ((int)blockIdx.x >= a.mass_wgs) {
+        const size_t row = blockIdx.x - a.mass_wgs, at = row * a.slots;
+        const SlotFactors s = slot_factors(a.pm, a.pl, at, a.slots, lane);
+        const float inv = s.L == 0.0f ? 0.0f : 1.0f / s.L;
+        __shared__ float f[2 * kSeqMaxSplits];
+        if (wave == 0) {
+            f[lane] = s.f0;
+            f[lane + 64] = s.f1;
         }
-    mass[(size_t)g * mass_stride + t] += sum;
+        __syncthreads();
+        const int sub = tid >> 5, d = 4 * (tid & 31);
+        f4 o = {0, 0, 0, 0};
+        if (d < a.hd) {
+            const float* p = a.po + at * a.hd + d;
+#pragma unroll 4
+            for (int t = sub; t < a.slots; t += 8) o += f[t] * *(const f4*)(p + (size_t)t * a.hd);
+        }
+        *(f4*)&red[sub][d] = o;
+        __syncthreads();
+        if (tid < a.hd) {
+            float x = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 8; t++) x += red[t][tid];
+            a.out[row * a.hd + tid] = s.L == 0.0f ? 0.0f : x * inv;
+        }
+        return;
+    }
+    __shared__ float2 ml[kMassRows];  // base, 1 / sum
+    const int g = blockIdx.x % a.n_kv, t = (blockIdx.x / a.n_kv) * 512 + 2 * tid;
+    const int rows = a.n * a.r;
+    float s0 = 0.0f, s1 = 0.0f;
+    for (int r0 = 0; r0 < rows; r0 += kMassRows) {
+        const int m = min(kMassRows, rows - r0);
+        __syncthreads();
+        for (int q = wave; q < m; q += 4) {
+            const int i = (r0 + q) / a.r;
+            const size_t row = (size_t)i * a.n_heads + g * a.r + (r0 + q - i * a.r);
+            const SlotFactors s = slot_factors(a.pm, a.pl, row * a.slots, a.slots, lane);
+            if (lane == 0) ml[q] = make_float2(s.L == 0.0f ? 0.0f : s.M, s.L == 0.0f ? 0.0f : 1.0f / s.L);
+        }
+        __syncthreads();
+        if (t < a.len) {
+#pragma unroll 8
+            for (int q = 0; q < m; q++) {
+                const int i = (r0 + q) / a.r;
+                const size_t row = (size_t)i * a.n_heads + g * a.r + (r0 + q - i * a.r);
+                const float2 x = *(const float2*)(a.scores + row * a.sstride + t), b = ml[q];
+                s0 = fmaf(__builtin_amdgcn_exp2f(x.x - b.x), b.y, s0);
+                s1 = fmaf(__builtin_amdgcn_exp2f(x.y - b.x), b.y, s1);
+            }
+        }
+    }
+    float* to = a.mass + (size_t)g * a.mass_stride + t;
+    if (t < a.len) to[0] += s0;
+    if (t + 1 < a.len) to[1] += s1;
 }
 
 template <int NQ, int RW>
@@ -558,6 +600,23 @@ static SeqArgs seq_args(const gllm_hip_kv* kv, int l, const float* d_q, int n, i
     return a;
 }
 
+static MergeArgs merge_args(const SeqArgs& a, const SeqPlan& p, float* d_out) {
+    MergeArgs m{};
+    m.pm = a.pm;
+    m.pl = a.pl;
+    m.po = a.po;
+    m.out = d_out;
+    m.rows = (int)p.rows;
+    m.slots = p.slots;
+    m.hd = a.hd;
+    m.n = a.n;
+    m.n_heads = a.n_heads;
+    m.n_kv = a.n_kv;
+    m.r = a.r;
+    m.len = a.len;
+    return m;
+}
+
 static int seq_launch(SeqArgs a, const SeqPlan& p, hipStream_t s) {
     a.shared_wgs = a.n_kv * p.row_blocks * p.chunks;
     a.slot0 = p.chunks;
@@ -603,8 +662,7 @@ int gllm_hip_attend_shared_dev(gllm_hip_kv* kv, int l, const float* d_q, int n, 
     a.starts = d_starts;
     a.lens = d_lens;
     GLLM_TRY(seq_launch(a, p, s));
-    hipLaunchKernelGGL(seq_merge_kernel, dim3((unsigned)((p.rows + 3) / 4)), dim3(256), 0, s, a.pm, a.pl, a.po, (int)p.rows, p.slots, hd, d_out,
-                       (float*)nullptr);
+    hipLaunchKernelGGL(seq_merge_kernel, dim3((unsigned)p.rows), dim3(256), 0, s, merge_args(a, p, d_out));
     GLLM_HIP(hipGetLastError());
     return GLLM_OK;
 }
@@ -630,18 +688,20 @@ int gllm_hip_attend_mass_dev(gllm_hip_kv* kv, int l, const float* d_q, int n, in
     const SeqPlan p = seq_plan(n, n_heads, n_kv_heads, len, 0);
     float* w;
     GLLM_TRY(seq_work(what, kv, seq_floats(p, hd, sstride), d_work, work_bytes, s, &w));
-    float* ml = w + p.rows * (size_t)sstride;
-    SeqArgs a = seq_args(kv, l, d_q, n, n_heads, n_kv_heads, hd, scale, p, ml + (p.rows * 2 + 3) / 4 * 4);
+    SeqArgs a = seq_args(kv, l, d_q, n, n_heads, n_kv_heads, hd, scale, p, w + p.rows * (size_t)sstride);
     a.start = start;
     a.len = len;
     a.causal = 1;
     a.scores = w;
     a.sstride = sstride;
     GLLM_TRY(seq_launch(a, p, s));
-    hipLaunchKernelGGL(seq_merge_kernel, dim3((unsigned)((p.rows + 3) / 4)), dim3(256), 0, s, a.pm, a.pl, a.po, (int)p.rows, p.slots, hd, d_out, ml);
-    GLLM_HIP(hipGetLastError());
-    hipLaunchKernelGGL(seq_mass_kernel, dim3((len + 255) / 256, n_kv_heads), dim3(256), 0, s, w, sstride, ml, n, n_heads,
-                       p.r, len, d_mass + start, mass_stride);
+    MergeArgs m = merge_args(a, p, d_out);
+    m.scores = w;
+    m.sstride = sstride;
+    m.mass = d_mass + start;
+    m.mass_stride = mass_stride;
+    m.mass_wgs = n_kv_heads * ((len + 511) / 512);
+    hipLaunchKernelGGL(seq_merge_kernel, dim3((unsigned)(m.mass_wgs + p.rows)), dim3(256), 0, s, m);
     GLLM_HIP(hipGetLastError());
     return GLLM_OK;
 }

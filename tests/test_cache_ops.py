@@ -41,7 +41,7 @@ int main() {
         }
         if (most) need(p.own_blocks * 16 >= r, "own blocks", n, h, g, len, most);
         need(seq_floats(p, 128, 0) >= p.rows * (size_t)p.slots * 130, "floats", n, h, g, len, most);
-        need(seq_floats(p, 128, 64) >= p.rows * (size_t)p.slots * 130 + p.rows * 66, "scored", n, h, g, len, most);
+        need(seq_floats(p, 128, 64) >= p.rows * (size_t)p.slots * 130 + p.rows * 64, "scored", n, h, g, len, most);
     }
     const int big = 2147483647;
     struct { int s, l, m, a, b; } cut[] = {{0, 5, 10, 0, 5}, {7, 5, 10, 7, 10}, {-3, 5, 10, 0, 2}, {-9, 5, 10, 0, 0}, {12, 5, 10, 10, 10},
