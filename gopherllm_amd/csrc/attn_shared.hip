@@ -5,15 +5,15 @@
 // model.go:1516); these serve callers that batch or bound it.
 //
 //   t_p   = (q . k_p) * scale * log2(e)
-//   w_p   = 2^(t_p - base)            base = (running maximum of t) - 15
+//   w_p   = 2^(t_p - base)            base: 8 to 15 below the running maximum of t
 //   out   = sum w_p v_p / sum w_p     over the shared rows, then the own rows
 //
 // K and V are f16 and q and w are float32.  Each of q and w is the sum of two
 // f16 values (its rounding and the rounding of the rest, 22 bits), so two
 // f16 matrix products, whose products are exact in the float32 accumulator,
 // stand for one float32 product at an eighth of its matrix-core time.  q is
-// first scaled by a power of two to a maximum in [2^14, 2^15), and the
-// weights by 2^15 (the 15 in base), so that the second part stays normal.
+// first scaled by a power of two to a maximum in [2^14, 2^15), and base lifts
+// the weights, so that the second part stays normal where it counts.
 //
 // A workgroup's four waves split the positions of a chunk, or its query rows
 // where there are many.  Per 32 positions a wave forms the transposed scores S^T = K Q^T and the transposed output
@@ -57,7 +57,10 @@ struct SeqArgs {
     int sstride;
 };
 
-constexpr float kSeqLift = 15.0f;
+// A new base puts the largest weight so far at 2^8; it stays until a weight
+// would pass 2^15, so that most steps leave the sums as they are (f16 ends at
+// 2^16; at the other end a weight's second part ends 2^-32 below the largest).
+constexpr float kSeqLift = 8.0f, kSeqRoom = 15.0f;
 constexpr int kBufferWord3 = 0x00020000;  // raw buffer of 32-bit data; reads past its end give 0
 
 // Bytes between rows of an LDS tile.  K rows are read 16 bytes a lane, eight
@@ -305,21 +308,24 @@ __device__ __forceinline__ void seq_run(const SeqArgs& a, int b, char* lds, floa
                     }
                 }
             }
-            mx = fmaxf(mx, __shfl_xor(mx, 16));
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const float nb = mx == ninf ? base[nq] : fmaxf(base[nq], mx * c[nq] - kSeqLift);
-            if (__any(nb > base[nq])) {
-                const float f = nb == base[nq] ? 1.0f : __builtin_amdgcn_exp2f(base[nq] - nb);
-                l[nq] *= f;
+            // a lane whose scores pass what its base allows: all lanes of a query agree on a new one
+            if (__any(mx * c[nq] - base[nq] > kSeqRoom)) {
+                mx = fmaxf(mx, __shfl_xor(mx, 16));
+                mx = fmaxf(mx, __shfl_xor(mx, 32));
+                const float top = mx * c[nq];
+                if (top - base[nq] > kSeqRoom) {
+                    const float nb = top - kSeqLift, f = __builtin_amdgcn_exp2f(base[nq] - nb);
+                    l[nq] *= f;
 #pragma unroll
-                for (int dt = 0; dt < DT; dt++) o[nq][dt] *= f;
-                base[nq] = nb;
+                    for (int dt = 0; dt < DT; dt++) o[nq][dt] *= f;
+                    base[nq] = nb;
+                }
             }
             f4 w[ST];
 #pragma unroll
             for (int t = 0; t < ST; t++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) w[t][j] = __builtin_amdgcn_exp2f(fmaf(s[nq][t][j], c[nq], -nb));
+                for (int j = 0; j < 4; j++) w[t][j] = __builtin_amdgcn_exp2f(fmaf(s[nq][t][j], c[nq], -base[nq]));
             if (!open) {
 #pragma unroll
                 for (int t = 0; t < ST; t++)
