@@ -61,6 +61,7 @@ struct SeqArgs {
 // would pass 2^15, so that most steps leave the sums as they are (f16 ends at
 // 2^16; at the other end a weight's second part ends 2^-32 below the largest).
 constexpr float kSeqLift = 8.0f, kSeqRoom = 15.0f;
+constexpr float kNoBase = -3.0e38f;  // of a query without positions so far: every factor of its zero sums is finite
 constexpr int kBufferWord3 = 0x00020000;  // raw buffer of 32-bit data; reads past its end give 0
 
 // Bytes between rows of an LDS tile.  K rows are read 16 bytes a lane, eight
@@ -76,7 +77,7 @@ struct Lds {
 template <int HD, int NQ, int RW>
 struct SeqShape {
     static constexpr int PW = kSeqWaves / RW;                // position groups
-    static constexpr int STEP = RW == 4 ? 64 : 32;           // positions of a step
+    static constexpr int STEP = RW == 4 && HD % 64 ? 64 : 32;           // positions of a step
     static constexpr int TILE = STEP * ((RW > 1 ? Lds<HD>::k_row : 0) + Lds<HD>::v_row);
     static constexpr int BUFS = RW > 1 ? 2 : 1;
     static constexpr int MERGE = PW > 1 ? kSeqWaves * 16 * (HD + 4) * 4 : 0;
@@ -219,7 +220,7 @@ __device__ __forceinline__ void seq_run(const SeqArgs& a, int b, char* lds, floa
     float base[NQ], l[NQ];
 #pragma unroll
     for (int nq = 0; nq < NQ; nq++) {
-        base[nq] = ninf;
+        base[nq] = kNoBase;
         l[nq] = 0.0f;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) o[nq][dt] = f4{0, 0, 0, 0};
@@ -276,82 +277,81 @@ __device__ __forceinline__ void seq_run(const SeqArgs& a, int b, char* lds, floa
             }
         }
         if (RW == 1 && more) load_k(pb + STEP);
-        h8 wh[NQ][ST / 2], wl[NQ][ST / 2];
-        const bool open = pb + STEP <= min(p1, lim_all);  // nothing in the tile is masked
+        // where the tile holds masked positions, scaled scores with -Inf in their places
+        float cc[NQ];
 #pragma unroll
-        for (int nq = 0; nq < NQ; nq++) {
-            float mx = ninf;
-            if (open) {
+        for (int nq = 0; nq < NQ; nq++) cc[nq] = c[nq];
+        if (pb + STEP > min(p1, lim_all)) {
 #pragma unroll
-                for (int t = 0; t < ST; t++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) mx = fmaxf(mx, s[nq][t][j]);
-            } else {
+            for (int nq = 0; nq < NQ; nq++) {
+                cc[nq] = 1.0f;
 #pragma unroll
                 for (int t = 0; t < ST; t++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (pb + 16 * t + 4 * grp + j < lim[nq]) mx = fmaxf(mx, s[nq][t][j]);
+                    for (int j = 0; j < 4; j++) s[nq][t][j] = pb + 16 * t + 4 * grp + j < lim[nq] ? s[nq][t][j] * c[nq] : ninf;
             }
-            if (!OWN && a.scores) {
+        }
+        if (!OWN && a.scores) {
+#pragma unroll
+            for (int nq = 0; nq < NQ; nq++) {
                 const int rr = row0 + 16 * nq + col;
                 if (rr < rows) {
                     const int i = rr / a.r;
                     float* to = a.scores + ((size_t)i * a.n_heads + g * a.r + (rr - i * a.r)) * a.sstride - a.start;
 #pragma unroll
-                    for (int t = 0; t < ST; t++) {
-                        const int pos = pb + 16 * t + 4 * grp;
-                        f4 x;
-#pragma unroll
-                        for (int j = 0; j < 4; j++) x[j] = pos + j < lim[nq] ? s[nq][t][j] * c[nq] : ninf;
-                        if (pos < p1) *(f4*)(to + pos) = x;
-                    }
+                    for (int t = 0; t < ST; t++)
+                        if (pb + 16 * t + 4 * grp < p1) *(f4*)(to + pb + 16 * t + 4 * grp) = s[nq][t] * cc[nq];
                 }
             }
-            // a lane whose scores pass what its base allows: all lanes of a query agree on a new one
-            if (__any(mx * c[nq] - base[nq] > kSeqRoom)) {
-                mx = fmaxf(mx, __shfl_xor(mx, 16));
-                mx = fmaxf(mx, __shfl_xor(mx, 32));
-                const float top = mx * c[nq];
-                if (top - base[nq] > kSeqRoom) {
-                    const float nb = top - kSeqLift, f = __builtin_amdgcn_exp2f(base[nq] - nb);
-                    l[nq] *= f;
-#pragma unroll
-                    for (int dt = 0; dt < DT; dt++) o[nq][dt] *= f;
-                    base[nq] = nb;
-                }
-            }
-            f4 w[ST];
-#pragma unroll
-            for (int t = 0; t < ST; t++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) w[t][j] = __builtin_amdgcn_exp2f(fmaf(s[nq][t][j], c[nq], -base[nq]));
-            if (!open) {
-#pragma unroll
-                for (int t = 0; t < ST; t++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (!(pb + 16 * t + 4 * grp + j < lim[nq])) w[t][j] = 0.0f;
-            }
-            // the two parts of a weight, both cut short: 21 bits
-#pragma unroll
-            for (int t = 0; t < ST; t++)
-#pragma unroll
-                for (int j = 0; j < 4; j += 2) {
-                    l[nq] += w[t][j] + w[t][j + 1];
-                    const auto hi = __builtin_amdgcn_cvt_pkrtz(w[t][j], w[t][j + 1]);
-                    const auto lo = __builtin_amdgcn_cvt_pkrtz(fmaf((float)hi[0], minus1, w[t][j]), fmaf((float)hi[1], minus1, w[t][j + 1]));
-                    const int at = 4 * (t & 1) + j;
-                    wh[nq][t / 2][at] = (_Float16)hi[0];
-                    wh[nq][t / 2][at + 1] = (_Float16)hi[1];
-                    wl[nq][t / 2][at] = (_Float16)lo[0];
-                    wl[nq][t / 2][at + 1] = (_Float16)lo[1];
-                }
         }
-        // operand k = 8 grp + 4 t + j of step u is position 32 u + 16 t + 4 grp + j
+        // a query whose scores pass what its base allows gets a new one
+        float mx[NQ];
+        bool over = false;
+#pragma unroll
+        for (int nq = 0; nq < NQ; nq++) {
+            mx[nq] = ninf;
+#pragma unroll
+            for (int t = 0; t < ST; t++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) mx[nq] = fmaxf(mx[nq], s[nq][t][j]);
+            over |= mx[nq] * cc[nq] - base[nq] > kSeqRoom;
+        }
+        if (__any(over)) {
+#pragma unroll
+            for (int nq = 0; nq < NQ; nq++) {
+                float top = fmaxf(mx[nq], __shfl_xor(mx[nq], 16));
+                top = fmaxf(top, __shfl_xor(top, 32)) * cc[nq];
+                const float nb = top - base[nq] > kSeqRoom ? top - kSeqLift : base[nq];
+                const float f = __builtin_amdgcn_exp2f(base[nq] - nb);
+                l[nq] *= f;
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) o[nq][dt] *= f;
+                base[nq] = nb;
+            }
+        }
+        // V operand k = 8 grp + 4 t + j of step u is position 32 u + 16 t + 4 grp + j
         const char* vt = cur + (RW > 1 ? STEP * Lds<HD>::k_row : 0) + (4 * grp + (col >> 2)) * Lds<HD>::v_row + 8 * (col & 3);
 #pragma unroll
-        for (int u = 0; u < ST / 2; u++)
+        for (int u = 0; u < ST / 2; u++) {
+            h8 wh[NQ], wl[NQ];
+#pragma unroll
+            for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int j = 0; j < 4; j += 2) {
+                        // the two parts of a weight, both cut short: 21 bits
+                        const f4 x = s[nq][2 * u + t];
+                        const float w0 = __builtin_amdgcn_exp2f(fmaf(x[j], cc[nq], -base[nq]));
+                        const float w1 = __builtin_amdgcn_exp2f(fmaf(x[j + 1], cc[nq], -base[nq]));
+                        l[nq] += w0 + w1;
+                        const auto hi = __builtin_amdgcn_cvt_pkrtz(w0, w1);
+                        const auto lo = __builtin_amdgcn_cvt_pkrtz(fmaf((float)hi[0], minus1, w0), fmaf((float)hi[1], minus1, w1));
+                        wh[nq][4 * t + j] = (_Float16)hi[0];
+                        wh[nq][4 * t + j + 1] = (_Float16)hi[1];
+                        wl[nq][4 * t + j] = (_Float16)lo[0];
+                        wl[nq][4 * t + j + 1] = (_Float16)lo[1];
+                    }
 #pragma unroll
             for (int dt = 0; dt < DT; dt++) {
                 s4 x[2];
@@ -361,10 +361,11 @@ __device__ __forceinline__ void seq_run(const SeqArgs& a, int b, char* lds, floa
                         (__attribute__((address_space(3))) s4*)(vt + (32 * u + 16 * t) * Lds<HD>::v_row + 32 * dt));
                 const h8 vf = join(x[0], x[1]);
 #pragma unroll
-                for (int nq = 0; nq < NQ; nq++) o[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, wl[nq][u], o[nq][dt], 0, 0, 0);
+                for (int nq = 0; nq < NQ; nq++) o[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, wl[nq], o[nq][dt], 0, 0, 0);
 #pragma unroll
-                for (int nq = 0; nq < NQ; nq++) o[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, wh[nq][u], o[nq][dt], 0, 0, 0);
+                for (int nq = 0; nq < NQ; nq++) o[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, wh[nq], o[nq][dt], 0, 0, 0);
             }
+        }
         asm volatile("" ::: "memory");
         if (RW > 1) {
             if (more) store_tile(tile + ((it + 1) & 1) * S::TILE);
@@ -407,13 +408,12 @@ __device__ __forceinline__ void seq_run(const SeqArgs& a, int b, char* lds, floa
 #pragma unroll
         for (int q = 0; q < RW; q++) {
             const int row = threadIdx.x >> 4, rr = (rb * RW + q) * 16 * NQ + 16 * nq + row;
-            float M = ninf, L = 0.0f, f[PW];
+            float M = kNoBase, L = 0.0f, f[PW];
 #pragma unroll
             for (int w = 0; w < PW; w++) M = fmaxf(M, sm[w * RW + q][row]);
 #pragma unroll
             for (int w = 0; w < PW; w++) {
-                const float m = sm[w * RW + q][row];
-                f[w] = m == ninf ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+                f[w] = __builtin_amdgcn_exp2f(sm[w * RW + q][row] - M);
                 L = fmaf(sl[w * RW + q][row], f[w], L);
             }
             if (rr < rows) {
@@ -452,13 +452,12 @@ struct SlotFactors {
 };
 __device__ __forceinline__ SlotFactors slot_factors(const float* pm, const float* pl, size_t at, int slots, int lane) {
     static_assert(2 * kSeqMaxSplits == 128, "two slots a lane");
-    const float ninf = -__int_as_float(0x7f800000);
-    const float m0 = lane < slots ? pm[at + lane] : ninf, m1 = lane + 64 < slots ? pm[at + lane + 64] : ninf;
+    const float m0 = lane < slots ? pm[at + lane] : kNoBase, m1 = lane + 64 < slots ? pm[at + lane + 64] : kNoBase;
     const float l0 = lane < slots ? pl[at + lane] : 0.0f, l1 = lane + 64 < slots ? pl[at + lane + 64] : 0.0f;
     SlotFactors r;
     r.M = wave_max(fmaxf(m0, m1));
-    r.f0 = m0 == ninf ? 0.0f : __builtin_amdgcn_exp2f(m0 - r.M);
-    r.f1 = m1 == ninf ? 0.0f : __builtin_amdgcn_exp2f(m1 - r.M);
+    r.f0 = __builtin_amdgcn_exp2f(m0 - r.M);
+    r.f1 = __builtin_amdgcn_exp2f(m1 - r.M);
     r.L = fmaf(l0, r.f0, l1 * r.f1);
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) r.L += __shfl_xor(r.L, off);
