@@ -32,8 +32,8 @@ inline SeqPlan seq_plan(int n, int n_heads, int n_kv, int len, int most) {
     p.r = n_heads / n_kv;
     p.rows = (size_t)n * n_heads;
     const long long per_kv = (long long)n * p.r;
-    p.nq = per_kv <= 32 ? 1 : 2;
-    p.rw = per_kv <= 16 ? 1 : per_kv <= 64 ? 2 : 4;
+    p.nq = per_kv <= 64 ? 1 : 2;
+    p.rw = per_kv <= 16 ? 1 : kSeqWaves;
     p.row_blocks = (int)((per_kv + 16 * p.nq * p.rw - 1) / (16 * p.nq * p.rw));
     if (len > 0) {
         const long long per_chunk = (long long)n_kv * p.row_blocks;

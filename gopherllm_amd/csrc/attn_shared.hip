@@ -64,124 +64,53 @@ constexpr float kSeqLift = 8.0f, kSeqRoom = 15.0f;
 constexpr float kNoBase = -3.0e38f;  // of a query without positions so far: every factor of its zero sums is finite
 constexpr int kBufferWord3 = 0x00020000;  // raw buffer of 32-bit data; reads past its end give 0
 
-// Bytes between rows of an LDS tile.  K rows are read 16 bytes a lane, eight
-// rows at a time: 16 bytes of padding spread them over the banks.  V rows are
-// read 32 bytes a row, four rows at a time, by the transposing loads: rows of
-// 256 and 128 bytes need 32 bytes of padding, 192 and 64 spread by themselves.
+// 16-byte chunk c of row r of an LDS tile lies at chunk c ^ f(r) of that row, so
+// that the eight rows of a phase of 16-byte reads (K) and the four rows of 32
+// bytes of a phase of transposing reads (V) meet different banks.
 template <int HD>
-struct Lds {
-    static constexpr int k_row = HD * 2 + 16;
-    static constexpr int v_row = HD * 2 + (HD % 64 == 0 ? 32 : 0);
-};
-
-template <int HD, int NQ, int RW>
-struct SeqShape {
-    static constexpr int PW = kSeqWaves / RW;                // position groups
-    static constexpr int STEP = RW == 4 && HD % 64 ? 64 : 32;           // positions of a step
-    static constexpr int TILE = STEP * ((RW > 1 ? Lds<HD>::k_row : 0) + Lds<HD>::v_row);
-    static constexpr int BUFS = RW > 1 ? 2 : 1;
-    static constexpr int MERGE = PW > 1 ? kSeqWaves * 16 * (HD + 4) * 4 : 0;
-    static constexpr int BYTES = PW * BUFS * TILE > MERGE ? PW * BUFS * TILE : MERGE;
-};
-
-__device__ __forceinline__ h8 join(s4 a, s4 b) {
-    h8 r;
-    const h4 x = __builtin_bit_cast(h4, a), y = __builtin_bit_cast(h4, b);
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        r[j] = x[j];
-        r[4 + j] = y[j];
-    }
-    return r;
+__device__ __forceinline__ int k_swizzle(int r) {
+    return HD % 64 == 0 ? r & 7 : (r >> 1) & 3;
+}
+template <int HD>
+__device__ __forceinline__ int v_swizzle(int r) {
+    return HD % 64 == 0 ? 2 * (r & 3) : 2 * ((r >> 1) & 1);
 }
 
-// HD: head size rounded up to 32 (hd <= HD, hd % 8 == 0); NQ: tiles of 16
-// query rows of a wave; RW: waves that take different query rows over the same
-// positions, sharing the K and V tiles; the kSeqWaves / RW groups of such waves
-// take different positions.  OWN: each token's own rows, not the shared ones.
-template <int HD, int NQ, int RW, bool OWN>
-__device__ __forceinline__ void seq_run(const SeqArgs& a, int b, char* lds, float (*sm)[16], float (*sl)[16]) {
-    using S = SeqShape<HD, NQ, RW>;
-    constexpr int KK = HD / 32, DT = HD / 16, CH = HD / 8, PW = S::PW, STEP = S::STEP, ST = STEP / 16;
-    constexpr int GT = RW * 64;                    // threads of a position group
-    constexpr int LD = STEP * CH / GT;             // 16-byte loads of a thread for a tile
-    static_assert(STEP * CH % GT == 0, "a tile is a whole number of loads");
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 15, grp = lane >> 4;
-    const int pg = wave / RW, rw = wave % RW;
-    const float ninf = -__int_as_float(0x7f800000);
+constexpr int kStep = 32;    // positions of a step
+constexpr int kStages = 4;   // tiles of the ring that row waves share, three of them on their way
 
-    const int g = b % a.n_kv;
-    b /= a.n_kv;
-    int rb, slot, tok = 0, a0, a1;  // rows a0 .. a1 - 1 of the cache
-    if (OWN) {
-        rb = b % a.own_blocks;
-        b /= a.own_blocks;
-        tok = b % a.n;
-        slot = b / a.n;
-        const RowSpan s = clip_rows(a.starts[tok], a.lens[tok], a.max_len);
-        const int chunk = (((s.b - s.a) + a.splits - 1) / a.splits + kSeqQuantum - 1) / kSeqQuantum * kSeqQuantum;
-        a0 = min(s.b, s.a + slot * chunk);
-        a1 = min(s.b, a0 + chunk);
-    } else {
-        rb = b % a.row_blocks;
-        slot = b / a.row_blocks;
-        a0 = a.start + slot * a.chunk;
-        a1 = min(a.start + a.len, a0 + a.chunk);
-    }
-    const int part = ((a1 - a0 + PW * STEP - 1) / (PW * STEP)) * STEP;  // positions of a group
-    const int p0 = min(a1, a0 + pg * part), p1 = min(a1, p0 + part);
+template <int HD, int RW>
+struct SeqLds {
+    static constexpr int TILE = kStep * HD * 2;  // bytes of K or V of a step
+    static constexpr int MERGE = kSeqWaves * 16 * (HD + 4) * 4;
+    static constexpr int OWN = kSeqWaves * TILE > MERGE ? kSeqWaves * TILE : MERGE;
+    static constexpr int RING = RW > 1 ? kStages * 2 * TILE : 0;
+    static constexpr int BYTES = RING > OWN ? RING : OWN;
+};
 
-    // A tile's K and V as loads.  V, and K where waves share it, go to LDS: 16-byte
-    // chunk e = GT u + thread of the group; K of a wave's own goes straight into
-    // operand order, u = t * KK + kk: position 16 t + col, dims 32 kk + 8 grp.
-    // The buffer ends with the range's last row, so what is past it reads as
-    // zero without a branch (V has to: the weight there is 0, and 0 * Inf is not);
-    // dims past hd get an offset past any buffer.
-    const int gt = rw * 64 + lane;
-    u4 kr[LD], vr[LD];
-    const auto rsrc = [&](const uint16_t* base, int kd, int pb) {
-        const int n = min(p1 - pb, STEP);
-        return __builtin_amdgcn_make_buffer_rsrc((void*)(base + (size_t)pb * kd + g * a.hd), 0,
-                                                 n > 0 ? ((n - 1) * kd + a.hd) * 2 : 0, kBufferWord3);
-    };
-    const auto chunk_off = [&](int u, int kd) {
-        const int e = GT * u + gt, d = 8 * (e % CH);
-        return d < a.hd ? (e / CH * kd + d) * 2 : (int)0x80000000;
-    };
-    const auto load_k = [&](int pb) {
-        const auto r = rsrc(a.K, a.kd_k, pb);
-#pragma unroll
-        for (int u = 0; u < LD; u++) {
-            const int t = u / KK, d = 32 * (u % KK) + 8 * grp;
-            const int off = RW > 1 ? chunk_off(u, a.kd_k) : d < a.hd ? ((16 * t + col) * a.kd_k + d) * 2 : (int)0x80000000;
-            kr[u] = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
-        }
-    };
-    const auto load_v = [&](int pb) {
-        const auto r = rsrc(a.V, a.kd_v, pb);
-#pragma unroll
-        for (int u = 0; u < LD; u++) vr[u] = __builtin_amdgcn_raw_buffer_load_b128(r, chunk_off(u, a.kd_v), 0, 0);
-    };
-    const int steps = part / STEP;  // the same for every wave of the workgroup
-    if (steps > 0) {  // on their way while the query rows are read and split
-        load_v(p0);
-        load_k(p0);
-    }
-
-    // query rows: rb * 16 * NQ * RW + 16 * (rw * NQ + nq) + col of this kv head
-    const int rows = OWN ? a.r : a.n * a.r;
-    const int row0 = (rb * RW + rw) * 16 * NQ;
-    h8 qh[NQ][KK], ql[NQ][KK];
+// NQ tiles of 16 query rows, one row a lane (col = lane & 15), dims 32 kk + 8 grp.
+template <int HD, int NQ>
+struct SeqRows {
+    h8 hi[NQ][HD / 32], lo[NQ][HD / 32];
     float c[NQ];
-    int lim[NQ];  // rows from it on are masked
+    int lim[NQ];  // cache rows from it on are masked
+    // and the sums so far: out^T tiles of 16 dims, base and sum of weights of this lane's positions
+    f4 o[NQ][HD / 16];
+    float base[NQ], l[NQ];
+};
+
+template <int HD, int NQ, bool OWN>
+__device__ __forceinline__ void seq_queries(const SeqArgs& a, int g, int tok, int row0, int p1, SeqRows<HD, NQ>& q) {
+    constexpr int KK = HD / 32;
+    const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+    const int rows = OWN ? a.r : a.n * a.r;
 #pragma unroll
     for (int nq = 0; nq < NQ; nq++) {
         const int rr = row0 + 16 * nq + col;
         const bool on = rr < rows;
         const int i = OWN ? tok : rr / a.r, hh = OWN ? rr : rr - i * a.r;
         const size_t row = on ? (size_t)i * a.n_heads + g * a.r + hh : 0;
-        lim[nq] = a.causal ? min(p1, a.start + a.len - (a.n - 1 - (on ? i : 0))) : p1;
+        q.lim[nq] = a.causal ? min(p1, a.start + a.len - (a.n - 1 - (on ? i : 0))) : p1;
         f4 x[KK][2];
         float mx = 0.0f;
 #pragma unroll
@@ -202,248 +131,376 @@ __device__ __forceinline__ void seq_run(const SeqArgs& a, int b, char* lds, floa
         int e = 15;
         if (mx > 0.0f && mx < __int_as_float(0x7f800000)) (void)frexpf(mx, &e);
         const int k = 15 - e;
-        c[nq] = ldexpf(fabsf(a.scale), -k);  // the sign goes into q, so a larger dot is a larger score
+        q.c[nq] = ldexpf(fabsf(a.scale), -k);  // the sign goes into q, so a larger dot is a larger score
 #pragma unroll
         for (int kk = 0; kk < KK; kk++)
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const float v = ldexpf(a.scale < 0.0f ? -x[kk][j >> 2][j & 3] : x[kk][j >> 2][j & 3], k);
                 const _Float16 hi = (_Float16)v;
-                qh[nq][kk][j] = hi;
-                ql[nq][kk][j] = (_Float16)(v - (float)hi);
+                q.hi[nq][kk][j] = hi;
+                q.lo[nq][kk][j] = (_Float16)(v - (float)hi);
             }
+        q.base[nq] = kNoBase;
+        q.l[nq] = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < HD / 16; dt++) q.o[nq][dt] = f4{0, 0, 0, 0};
     }
-    int lim_all = a1;  // rows that no row of this wave masks
-    if (!OWN && a.causal) lim_all = a.start + a.len - (a.n - 1 - min(row0 / a.r, a.n - 1));
+}
 
-    f4 o[NQ][DT];
-    float base[NQ], l[NQ];
+// s[nq][t] += K rows (16 positions of tile t) times the query rows
+template <int HD, int NQ>
+__device__ __forceinline__ void seq_dot(const h8 (&k)[HD / 32], const SeqRows<HD, NQ>& q, f4 (&s)[NQ][2], int t) {
 #pragma unroll
-    for (int nq = 0; nq < NQ; nq++) {
-        base[nq] = kNoBase;
-        l[nq] = 0.0f;
+    for (int nq = 0; nq < NQ; nq++) s[nq][t] = f4{0, 0, 0, 0};
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++) o[nq][dt] = f4{0, 0, 0, 0};
+    for (int kk = 0; kk < HD / 32; kk++) {
+#pragma unroll
+        for (int nq = 0; nq < NQ; nq++) s[nq][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[kk], q.lo[nq][kk], s[nq][t], 0, 0, 0);
+#pragma unroll
+        for (int nq = 0; nq < NQ; nq++) s[nq][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[kk], q.hi[nq][kk], s[nq][t], 0, 0, 0);
     }
+}
 
-    char* tile = lds + pg * S::BUFS * S::TILE;
-    const auto store_tile = [&](char* to) {
+// The step at position pb: scores s to weights, and the weighted rows of the V
+// tile at vt (LDS) added to the sums.  open: nothing in the step is masked.
+template <int HD, int NQ>
+__device__ __forceinline__ void seq_step(const SeqArgs& a, int g, int row0, int pb, int p1, bool open, bool scored,
+                                         f4 (&s)[NQ][2], SeqRows<HD, NQ>& q, const char* vt, float minus1) {
+    constexpr int DT = HD / 16;
+    const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+    const float ninf = -__int_as_float(0x7f800000);
+    // where the step holds masked positions, scaled scores with -Inf in their places
+    float cc[NQ];
 #pragma unroll
-        for (int u = 0; u < LD; u++) {
-            const int e = GT * u + gt, rr = e / CH, ch = e % CH;
-            if (RW > 1) *(u4*)(to + rr * Lds<HD>::k_row + 16 * ch) = kr[u];
-            *(u4*)(to + (RW > 1 ? STEP * Lds<HD>::k_row : 0) + rr * Lds<HD>::v_row + 16 * ch) = vr[u];
-        }
-    };
-
-    float minus1 = -1.0f;  // a register, so that w - hi is one mixed-precision fma of hi as it lies
-    asm volatile("" : "+v"(minus1));
-    if (RW > 1 && steps > 0) {
-        store_tile(tile);
-        __syncthreads();
-    }
-    for (int it = 0; it < steps; it++) {
-        const int pb = p0 + it * STEP;
-        const bool more = it + 1 < steps;
-        char* cur = tile + (RW > 1 ? (it & 1) * S::TILE : 0);
-        h8 kf[ST][KK];
-        if (RW == 1) {
-            if (pb >= p1) break;  // no barrier in this loop
-            store_tile(cur);
-            if (more) load_v(pb + STEP);
-#pragma unroll
-            for (int t = 0; t < ST; t++)
-#pragma unroll
-                for (int kk = 0; kk < KK; kk++) kf[t][kk] = __builtin_bit_cast(h8, kr[(t * KK + kk) % LD]);
-        } else {
-            if (more) {
-                load_k(pb + STEP);
-                load_v(pb + STEP);
-            }
-        }
-        f4 s[NQ][ST];
-#pragma unroll
-        for (int t = 0; t < ST; t++) {
-#pragma unroll
-            for (int nq = 0; nq < NQ; nq++) s[nq][t] = f4{0, 0, 0, 0};
-#pragma unroll
-            for (int kk = 0; kk < KK; kk++) {
-                const h8 k = RW == 1 ? kf[t][kk]
-                                     : *(const h8*)(cur + (16 * t + col) * Lds<HD>::k_row + 64 * kk + 16 * grp);
-#pragma unroll
-                for (int nq = 0; nq < NQ; nq++) s[nq][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[nq][kk], s[nq][t], 0, 0, 0);
-#pragma unroll
-                for (int nq = 0; nq < NQ; nq++) s[nq][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[nq][kk], s[nq][t], 0, 0, 0);
-            }
-        }
-        if (RW == 1 && more) load_k(pb + STEP);
-        // where the tile holds masked positions, scaled scores with -Inf in their places
-        float cc[NQ];
-#pragma unroll
-        for (int nq = 0; nq < NQ; nq++) cc[nq] = c[nq];
-        if (pb + STEP > min(p1, lim_all)) {
-#pragma unroll
-            for (int nq = 0; nq < NQ; nq++) {
-                cc[nq] = 1.0f;
-#pragma unroll
-                for (int t = 0; t < ST; t++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) s[nq][t][j] = pb + 16 * t + 4 * grp + j < lim[nq] ? s[nq][t][j] * c[nq] : ninf;
-            }
-        }
-        if (!OWN && a.scores) {
-#pragma unroll
-            for (int nq = 0; nq < NQ; nq++) {
-                const int rr = row0 + 16 * nq + col;
-                if (rr < rows) {
-                    const int i = rr / a.r;
-                    float* to = a.scores + ((size_t)i * a.n_heads + g * a.r + (rr - i * a.r)) * a.sstride - a.start;
-#pragma unroll
-                    for (int t = 0; t < ST; t++)
-                        if (pb + 16 * t + 4 * grp < p1) *(f4*)(to + pb + 16 * t + 4 * grp) = s[nq][t] * cc[nq];
-                }
-            }
-        }
-        // a query whose scores pass what its base allows gets a new one
-        float mx[NQ];
-        bool over = false;
+    for (int nq = 0; nq < NQ; nq++) cc[nq] = q.c[nq];
+    if (!open) {
 #pragma unroll
         for (int nq = 0; nq < NQ; nq++) {
-            mx[nq] = ninf;
+            cc[nq] = 1.0f;
 #pragma unroll
-            for (int t = 0; t < ST; t++)
+            for (int t = 0; t < 2; t++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) mx[nq] = fmaxf(mx[nq], s[nq][t][j]);
-            over |= mx[nq] * cc[nq] - base[nq] > kSeqRoom;
-        }
-        if (__any(over)) {
-#pragma unroll
-            for (int nq = 0; nq < NQ; nq++) {
-                float top = fmaxf(mx[nq], __shfl_xor(mx[nq], 16));
-                top = fmaxf(top, __shfl_xor(top, 32)) * cc[nq];
-                const float nb = top - base[nq] > kSeqRoom ? top - kSeqLift : base[nq];
-                const float f = __builtin_amdgcn_exp2f(base[nq] - nb);
-                l[nq] *= f;
-#pragma unroll
-                for (int dt = 0; dt < DT; dt++) o[nq][dt] *= f;
-                base[nq] = nb;
-            }
-        }
-        // V operand k = 8 grp + 4 t + j of step u is position 32 u + 16 t + 4 grp + j
-        const char* vt = cur + (RW > 1 ? STEP * Lds<HD>::k_row : 0) + (4 * grp + (col >> 2)) * Lds<HD>::v_row + 8 * (col & 3);
-#pragma unroll
-        for (int u = 0; u < ST / 2; u++) {
-            h8 wh[NQ], wl[NQ];
-#pragma unroll
-            for (int nq = 0; nq < NQ; nq++)
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int j = 0; j < 4; j += 2) {
-                        // the two parts of a weight, both cut short: 21 bits
-                        const f4 x = s[nq][2 * u + t];
-                        const float w0 = __builtin_amdgcn_exp2f(fmaf(x[j], cc[nq], -base[nq]));
-                        const float w1 = __builtin_amdgcn_exp2f(fmaf(x[j + 1], cc[nq], -base[nq]));
-                        l[nq] += w0 + w1;
-                        const auto hi = __builtin_amdgcn_cvt_pkrtz(w0, w1);
-                        const auto lo = __builtin_amdgcn_cvt_pkrtz(fmaf((float)hi[0], minus1, w0), fmaf((float)hi[1], minus1, w1));
-                        wh[nq][4 * t + j] = (_Float16)hi[0];
-                        wh[nq][4 * t + j + 1] = (_Float16)hi[1];
-                        wl[nq][4 * t + j] = (_Float16)lo[0];
-                        wl[nq][4 * t + j + 1] = (_Float16)lo[1];
-                    }
-#pragma unroll
-            for (int dt = 0; dt < DT; dt++) {
-                s4 x[2];
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-                    x[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) s4*)(vt + (32 * u + 16 * t) * Lds<HD>::v_row + 32 * dt));
-                const h8 vf = join(x[0], x[1]);
-#pragma unroll
-                for (int nq = 0; nq < NQ; nq++) o[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, wl[nq], o[nq][dt], 0, 0, 0);
-#pragma unroll
-                for (int nq = 0; nq < NQ; nq++) o[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, wh[nq], o[nq][dt], 0, 0, 0);
-            }
-        }
-        asm volatile("" ::: "memory");
-        if (RW > 1) {
-            if (more) store_tile(tile + ((it + 1) & 1) * S::TILE);
-            __syncthreads();
+                for (int j = 0; j < 4; j++) s[nq][t][j] = pb + 16 * t + 4 * grp + j < q.lim[nq] ? s[nq][t][j] * q.c[nq] : ninf;
         }
     }
-
-    // results: straight to the partials, or the position groups' joined in LDS,
-    // one tile of query rows of every row wave at a time
+    if (scored) {
+#pragma unroll
+        for (int nq = 0; nq < NQ; nq++) {
+            const int rr = row0 + 16 * nq + col;
+            if (rr < a.n * a.r) {
+                const int i = rr / a.r;
+                float* to = a.scores + ((size_t)i * a.n_heads + g * a.r + (rr - i * a.r)) * a.sstride - a.start;
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+                    if (pb + 16 * t + 4 * grp < p1) *(f4*)(to + pb + 16 * t + 4 * grp) = s[nq][t] * cc[nq];
+            }
+        }
+    }
+    // a query whose scores pass what its base allows gets a new one
+    float mx[NQ];
+    bool over = false;
 #pragma unroll
     for (int nq = 0; nq < NQ; nq++) {
-        float ls = l[nq];
+        mx[nq] = ninf;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) mx[nq] = fmaxf(mx[nq], s[nq][t][j]);
+        over |= mx[nq] * cc[nq] - q.base[nq] > kSeqRoom;
+    }
+    if (__any(over)) {
+#pragma unroll
+        for (int nq = 0; nq < NQ; nq++) {
+            float top = fmaxf(mx[nq], __shfl_xor(mx[nq], 16));
+            top = fmaxf(top, __shfl_xor(top, 32)) * cc[nq];
+            const float nb = top - q.base[nq] > kSeqRoom ? top - kSeqLift : q.base[nq];
+            const float f = __builtin_amdgcn_exp2f(q.base[nq] - nb);
+            q.l[nq] *= f;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) q.o[nq][dt] *= f;
+            q.base[nq] = nb;
+        }
+    }
+    h8 wh[NQ], wl[NQ];
+#pragma unroll
+    for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int j = 0; j < 4; j += 2) {
+                // the two parts of a weight, both cut short: 21 bits
+                const float w0 = __builtin_amdgcn_exp2f(fmaf(s[nq][t][j], cc[nq], -q.base[nq]));
+                const float w1 = __builtin_amdgcn_exp2f(fmaf(s[nq][t][j + 1], cc[nq], -q.base[nq]));
+                q.l[nq] += w0 + w1;
+                const auto hi = __builtin_amdgcn_cvt_pkrtz(w0, w1);
+                const auto lo = __builtin_amdgcn_cvt_pkrtz(fmaf((float)hi[0], minus1, w0), fmaf((float)hi[1], minus1, w1));
+                wh[nq][4 * t + j] = (_Float16)hi[0];
+                wh[nq][4 * t + j + 1] = (_Float16)hi[1];
+                wl[nq][4 * t + j] = (_Float16)lo[0];
+                wl[nq][4 * t + j + 1] = (_Float16)lo[1];
+            }
+    // V operand k = 8 grp + 4 t + j is position 16 t + 4 grp + j
+    const int vr = 4 * grp + (col >> 2);
+    const char* vp = vt + vr * HD * 2 + 8 * (col & 1);
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) {
+        s4 x[2];
+#pragma unroll
+        for (int t = 0; t < 2; t++)  // rows 16 apart share their swizzle
+            x[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(
+                vp + 16 * t * HD * 2 + 16 * ((2 * dt + ((col & 3) >> 1)) ^ v_swizzle<HD>(vr))));
+        h8 vf;
+        const h4 y0 = __builtin_bit_cast(h4, x[0]), y1 = __builtin_bit_cast(h4, x[1]);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            vf[j] = y0[j];
+            vf[4 + j] = y1[j];
+        }
+#pragma unroll
+        for (int nq = 0; nq < NQ; nq++) q.o[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, wl[nq], q.o[nq][dt], 0, 0, 0);
+#pragma unroll
+        for (int nq = 0; nq < NQ; nq++) q.o[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, wh[nq], q.o[nq][dt], 0, 0, 0);
+    }
+}
+
+// Rows pb .. min(pb + kStep, p1) - 1 of a kv head as a buffer: what is past its
+// end reads as zero without a branch (V has to: the weight there is 0, and
+// 0 * Inf is not).  A lane gives dims past hd an offset past any buffer.
+struct SeqBuffer {
+    const uint16_t* at;
+    int bytes;
+    __device__ __forceinline__ SeqBuffer(const uint16_t* base, int kd, int hd, int g, int pb, int p1) {
+        const int n = min(p1 - pb, kStep);
+        at = base + (size_t)pb * kd + g * hd;
+        bytes = n > 0 ? ((n - 1) * kd + hd) * 2 : 0;
+    }
+    __device__ __forceinline__ u4 words() const {
+        const uint64_t p = (uint64_t)at;
+        return u4{(uint32_t)p, (uint32_t)(p >> 32) & 0xFFFFu, (uint32_t)bytes, (uint32_t)kBufferWord3};
+    }
+    __device__ __forceinline__ u4 load(int off) const {
+        return __builtin_amdgcn_raw_buffer_load_b128(__builtin_amdgcn_make_buffer_rsrc((void*)at, 0, bytes, kBufferWord3), off, 0, 0);
+    }
+};
+constexpr int kPastEnd = (int)0x80000000;
+
+__device__ __forceinline__ size_t seq_part(const SeqArgs& a, bool own, int g, int tok, int rr, int slot) {
+    const int i = own ? tok : rr / a.r, hh = own ? rr : rr - i * a.r;
+    return ((size_t)i * a.n_heads + g * a.r + hh) * a.slots + slot + (own ? a.slot0 : 0);
+}
+
+// Up to 16 query rows: the four waves take different positions, each with K
+// straight from memory into operand order and V through its own LDS tile, and
+// join their sums in LDS.  HD: head size rounded up to 32 (hd <= HD,
+// hd % 8 == 0); OWN: each token's own rows, not the shared ones.
+template <int HD, bool OWN>
+__device__ __forceinline__ void seq_few(const SeqArgs& a, int b, char* lds, float (*sm)[16], float (*sl)[16]) {
+    constexpr int KK = HD / 32, DT = HD / 16, CH = HD / 8, LD = kStep * CH / 64;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, grp = lane >> 4;
+    const int g = b % a.n_kv;
+    b /= a.n_kv;
+    int rb, slot, tok = 0, a0, a1;  // rows a0 .. a1 - 1 of the cache
+    if (OWN) {
+        rb = b % a.own_blocks;
+        b /= a.own_blocks;
+        tok = b % a.n;
+        slot = b / a.n;
+        const RowSpan s = clip_rows(a.starts[tok], a.lens[tok], a.max_len);
+        const int chunk = (((s.b - s.a) + a.splits - 1) / a.splits + kSeqQuantum - 1) / kSeqQuantum * kSeqQuantum;
+        a0 = min(s.b, s.a + slot * chunk);
+        a1 = min(s.b, a0 + chunk);
+    } else {
+        rb = b % a.row_blocks;
+        slot = b / a.row_blocks;
+        a0 = a.start + slot * a.chunk;
+        a1 = min(a.start + a.len, a0 + a.chunk);
+    }
+    const int part = ((a1 - a0 + kSeqWaves * kStep - 1) / (kSeqWaves * kStep)) * kStep;  // positions of a wave
+    const int p0 = min(a1, a0 + wave * part), p1 = min(a1, p0 + part);
+    const int rows = OWN ? a.r : a.n * a.r, row0 = rb * 16;
+
+    u4 kr[2][KK], vr[LD];
+    const auto load_k = [&](int pb) {
+        const SeqBuffer r(a.K, a.kd_k, a.hd, g, pb, p1);
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++) {
+                const int d = 32 * kk + 8 * grp;
+                kr[t][kk] = r.load(d < a.hd ? ((16 * t + col) * a.kd_k + d) * 2 : kPastEnd);
+            }
+    };
+    const auto load_v = [&](int pb) {
+        const SeqBuffer r(a.V, a.kd_v, a.hd, g, pb, p1);
+#pragma unroll
+        for (int u = 0; u < LD; u++) {
+            const int e = 64 * u + lane, d = 8 * (e % CH);
+            vr[u] = r.load(d < a.hd ? (e / CH * a.kd_v + d) * 2 : kPastEnd);
+        }
+    };
+    if (p0 < p1) {  // on their way while the query rows are read and split
+        load_v(p0);
+        load_k(p0);
+    }
+    SeqRows<HD, 1> q;
+    seq_queries<HD, 1, OWN>(a, g, tok, row0, p1, q);
+    int lim_all = p1;  // positions that no row of this wave masks
+    if (!OWN && a.causal) lim_all = min(p1, a.start + a.len - (a.n - 1 - row0 / a.r));
+    float minus1 = -1.0f;  // a register, so that w - hi is one mixed-precision fma of hi as it lies
+    asm volatile("" : "+v"(minus1));
+    char* vt = lds + wave * SeqLds<HD, 1>::TILE;
+    for (int pb = p0; pb < p1; pb += kStep) {
+        const bool more = pb + kStep < p1;
+#pragma unroll
+        for (int u = 0; u < LD; u++) {
+            const int e = 64 * u + lane, rr = e / CH;
+            *(u4*)(vt + rr * HD * 2 + 16 * (e % CH ^ v_swizzle<HD>(rr))) = vr[u];
+        }
+        if (more) load_v(pb + kStep);
+        f4 s[1][2];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            h8 k[KK];
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++) k[kk] = __builtin_bit_cast(h8, kr[t][kk]);
+            seq_dot<HD, 1>(k, q, s, t);
+        }
+        if (more) load_k(pb + kStep);
+        seq_step<HD, 1>(a, g, row0, pb, p1, pb + kStep <= lim_all, !OWN && a.scores, s, q, vt, minus1);
+        asm volatile("" ::: "memory");
+    }
+
+    float ls = q.l[0];
+    ls += __shfl_xor(ls, 16);
+    ls += __shfl_xor(ls, 32);
+    float* so = (float*)lds;  // [wave][16][HD + 4]
+    __syncthreads();
+    if (grp == 0) {
+        sm[wave][col] = q.base[0];
+        sl[wave][col] = ls;
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) *(f4*)(so + (wave * 16 + col) * (HD + 4) + 16 * dt + 4 * grp) = q.o[0][dt];
+    __syncthreads();
+    // 16 threads a row, dims 4 (t % 16) + 64 v
+    const int row = threadIdx.x >> 4, rr = row0 + row;
+    if (rr >= rows) return;
+    float M = kNoBase, L = 0.0f, f[kSeqWaves];
+#pragma unroll
+    for (int w = 0; w < kSeqWaves; w++) M = fmaxf(M, sm[w][row]);
+#pragma unroll
+    for (int w = 0; w < kSeqWaves; w++) {
+        f[w] = __builtin_amdgcn_exp2f(sm[w][row] - M);
+        L = fmaf(sl[w][row], f[w], L);
+    }
+    const size_t at = seq_part(a, OWN, g, tok, rr, slot);
+    if ((threadIdx.x & 15) == 0) {
+        a.pm[at] = M;
+        a.pl[at] = L;
+    }
+    for (int d = 4 * (threadIdx.x & 15); d < a.hd; d += 64) {
+        f4 x = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < kSeqWaves; w++) x += f[w] * *(const f4*)(so + (w * 16 + row) * (HD + 4) + d);
+        *(f4*)(a.po + at * a.hd + d) = x;
+    }
+}
+
+// Many query rows: the four waves take 16 NQ rows each over the same positions
+// and share the K and V tiles, which direct copies bring into a ring of stages
+// three steps ahead (registers for one step ahead left the kernel waiting on
+// memory: 64 requests over 32768 rows took 85 us).
+template <int HD, int NQ>
+__device__ __forceinline__ void seq_many(const SeqArgs& a, int b, char* lds) {
+    constexpr int KK = HD / 32, DT = HD / 16, CH = HD / 8, TILE = SeqLds<HD, 4>::TILE;
+    constexpr int U = 2 * kStep * CH / 256;  // copies of a wave for a stage: 64 chunks each, K first, then V
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, grp = lane >> 4;
+    const int g = b % a.n_kv;
+    b /= a.n_kv;
+    const int rb = b % a.row_blocks, slot = b / a.row_blocks;
+    const int p0 = a.start + slot * a.chunk, p1 = min(a.start + a.len, p0 + a.chunk);
+    const int rows = a.n * a.r, row0 = (rb * kSeqWaves + wave) * 16 * NQ;
+
+    int off[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int w = kSeqWaves * u + wave, per = kStep * CH / 64;  // copy w of the stage
+        const bool v = w >= per;
+        const int e = 64 * (v ? w - per : w) + lane, r = e / CH, d = 8 * (e % CH ^ (v ? v_swizzle<HD>(r) : k_swizzle<HD>(r)));
+        off[u] = d < a.hd ? (r * (v ? a.kd_v : a.kd_k) + d) * 2 : kPastEnd;
+    }
+    const uint32_t ring = lds_addr(lds);
+    const auto copy = [&](int step) {  // past the last step the buffers are empty, and nothing is read
+        const int pb = min(p0 + step * kStep, p1);
+        const u4 k = SeqBuffer(a.K, a.kd_k, a.hd, g, pb, p1).words(), v = SeqBuffer(a.V, a.kd_v, a.hd, g, pb, p1).words();
+        const uint32_t to = ring + (step % kStages) * 2 * TILE;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int w = kSeqWaves * u + wave;
+            lds_buffer16(w >= kStep * CH / 64 ? v : k, off[u], to + 1024 * w);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; i++) copy(i);
+    SeqRows<HD, NQ> q;
+    seq_queries<HD, NQ, false>(a, g, 0, row0, p1, q);
+    int lim_all = p1;  // positions that no row of this wave masks
+    if (a.causal) lim_all = min(p1, a.start + a.len - (a.n - 1 - min(row0 / a.r, a.n - 1)));
+    float minus1 = -1.0f;  // a register, so that w - hi is one mixed-precision fma of hi as it lies
+    asm volatile("" : "+v"(minus1));
+    const int steps = (p1 - p0 + kStep - 1) / kStep;
+    for (int it = 0; it < steps; it++) {
+        // this wave's copies of the stage are in (two later stages may be out),
+        // and its reads of the stage before, whose place the next copies take
+        wait_vmem_le<2 * U>();
+        wait_lgkm0();
+        lds_barrier();
+        copy(it + kStages - 1);
+        const char* kt = lds + (it % kStages) * 2 * TILE;
+        f4 s[NQ][2];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            h8 k[KK];
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++)
+                k[kk] = *(const h8*)(kt + (16 * t + col) * HD * 2 + 16 * ((4 * kk + grp) ^ k_swizzle<HD>(col)));
+            seq_dot<HD, NQ>(k, q, s, t);
+        }
+        const int pb = p0 + it * kStep;
+        seq_step<HD, NQ>(a, g, row0, pb, p1, pb + kStep <= lim_all, a.scores != nullptr, s, q, kt + TILE, minus1);
+    }
+    wait_vmem_le<0>();  // no copy outlives the workgroup
+#pragma unroll
+    for (int nq = 0; nq < NQ; nq++) {
+        float ls = q.l[nq];
         ls += __shfl_xor(ls, 16);
         ls += __shfl_xor(ls, 32);
-        if (PW == 1) {
-            const int rr = row0 + 16 * nq + col;
-            if (rr < rows) {
-                const int i = OWN ? tok : rr / a.r, hh = OWN ? rr : rr - i * a.r;
-                const size_t at = ((size_t)i * a.n_heads + g * a.r + hh) * a.slots + slot + (OWN ? a.slot0 : 0);
-                if (grp == 0) {
-                    a.pm[at] = base[nq];
-                    a.pl[at] = ls;
-                }
-#pragma unroll
-                for (int dt = 0; dt < DT; dt++)
-                    if (16 * dt + 4 * grp < a.hd) *(f4*)(a.po + at * a.hd + 16 * dt + 4 * grp) = o[nq][dt];
+        const int rr = row0 + 16 * nq + col;
+        if (rr < rows) {
+            const size_t at = seq_part(a, false, g, 0, rr, slot);
+            if (grp == 0) {
+                a.pm[at] = q.base[nq];
+                a.pl[at] = ls;
             }
-            continue;
-        }
-        float* so = (float*)lds;  // [wave][16][HD + 4]
-        __syncthreads();
-        if (grp == 0) {
-            sm[wave][col] = base[nq];
-            sl[wave][col] = ls;
-        }
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++) *(f4*)(so + (wave * 16 + col) * (HD + 4) + 16 * dt + 4 * grp) = o[nq][dt];
-        __syncthreads();
-        // 16 threads a row: RW * 16 rows, dims 4 (t % 16) + 64 v
-#pragma unroll
-        for (int q = 0; q < RW; q++) {
-            const int row = threadIdx.x >> 4, rr = (rb * RW + q) * 16 * NQ + 16 * nq + row;
-            float M = kNoBase, L = 0.0f, f[PW];
-#pragma unroll
-            for (int w = 0; w < PW; w++) M = fmaxf(M, sm[w * RW + q][row]);
-#pragma unroll
-            for (int w = 0; w < PW; w++) {
-                f[w] = __builtin_amdgcn_exp2f(sm[w * RW + q][row] - M);
-                L = fmaf(sl[w * RW + q][row], f[w], L);
-            }
-            if (rr < rows) {
-                const int i = OWN ? tok : rr / a.r, hh = OWN ? rr : rr - i * a.r;
-                const size_t at = ((size_t)i * a.n_heads + g * a.r + hh) * a.slots + slot + (OWN ? a.slot0 : 0);
-                if ((threadIdx.x & 15) == 0) {
-                    a.pm[at] = M;
-                    a.pl[at] = L;
-                }
-                for (int d = 4 * (threadIdx.x & 15); d < a.hd; d += 64) {
-                    f4 x = {0, 0, 0, 0};
-#pragma unroll
-                    for (int w = 0; w < PW; w++) x += f[w] * *(const f4*)(so + ((w * RW + q) * 16 + row) * (HD + 4) + d);
-                    *(f4*)(a.po + at * a.hd + d) = x;
-                }
-            }
+            for (int dt = 0; dt < DT; dt++)
+                if (16 * dt + 4 * grp < a.hd) *(f4*)(a.po + at * a.hd + 16 * dt + 4 * grp) = q.o[nq][dt];
         }
     }
 }
 
-// Shared and own ranges in one launch: own_wgs workgroups of own ranges among
-// the shared ones.
+// Shared and own ranges in one launch, the shared ones first.
 template <int HD, int NQ, int RW>
 __global__ __launch_bounds__(256, 2) void seq_attend_kernel(SeqArgs a) {
-    constexpr int A = SeqShape<HD, NQ, RW>::BYTES, B = SeqShape<HD, 1, 1>::BYTES;
-    __shared__ __align__(16) char lds[A > B ? A : B];
+    __shared__ __align__(16) char lds[SeqLds<HD, RW>::BYTES];
     __shared__ float sm[kSeqWaves][16], sl[kSeqWaves][16];
     const int b = blockIdx.x;
-    if (b < a.shared_wgs) seq_run<HD, NQ, RW, false>(a, b, lds, sm, sl);
-    else seq_run<HD, 1, 1, true>(a, b - a.shared_wgs, lds, sm, sl);
+    if (b >= a.shared_wgs) seq_few<HD, true>(a, b - a.shared_wgs, lds, sm, sl);
+    else if constexpr (RW == 1) seq_few<HD, false>(a, b, lds, sm, sl);
+    else seq_many<HD, NQ>(a, b, lds);
 }
 
 // The factor of each of a row's slots (two a lane), and the row's base and sum.
@@ -628,8 +685,7 @@ static int seq_launch(SeqArgs a, const SeqPlan& p, hipStream_t s) {
     const long long blocks = a.shared_wgs + (long long)a.n_kv * p.own_blocks * a.n * p.splits;
     if (blocks == 0) return GLLM_OK;
     if (p.rw == 1) seq_launch_hd<1, 1>(a, (int)blocks, s);
-    else if (p.nq == 1) seq_launch_hd<1, 2>(a, (int)blocks, s);
-    else if (p.rw == 2) seq_launch_hd<2, 2>(a, (int)blocks, s);
+    else if (p.nq == 1) seq_launch_hd<1, 4>(a, (int)blocks, s);
     else seq_launch_hd<2, 4>(a, (int)blocks, s);
     GLLM_HIP(hipGetLastError());
     return GLLM_OK;

@@ -490,6 +490,16 @@ __device__ __forceinline__ void lds_copy4(const void* gsrc, uint32_t lds_dst) {
                  : "memory", "m0");
 }
 
+// The same from a buffer (its four resource words; lanes past its end write
+// zero).  Five wait states: one for M0, and five where a resource word comes
+// from a vector instruction.
+__device__ __forceinline__ void lds_buffer16(uint32_t __attribute__((ext_vector_type(4))) rsrc, int offset, uint32_t lds_dst) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+                 :
+                 : "v"(offset), "s"(rsrc), "s"(lds_dst)
+                 : "memory", "m0");
+}
+
 // s_waitcnt vmcnt(N) for a compile-time N (gfx9 encoding: vmcnt bits [3:0]
 // and [15:14], expcnt [6:4] and lgkmcnt [11:8] left unconstrained).
 template <int N>

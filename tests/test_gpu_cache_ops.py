@@ -168,6 +168,20 @@ def test_shared_query_magnitudes(hip, mag):
     assert np.abs(host(out)[0] - want).max() <= u * vm * (64 if mag < 1e-37 or mag > 1e38 else 1)
 
 
+@pytest.mark.parametrize("n,heads,n_kv,hd,length", [(40, 8, 2, 80, 45), (12, 8, 1, 72, 33), (3, 8, 2, 40, 70), (33, 16, 4, 120, 129), (64, 8, 2, 24, 1)])
+def test_shared_reads_nothing_left_in_lds(hip, n, heads, n_kv, hd, length):
+    """After a call that fills every LDS tile with NaN: head sizes and ranges that do not fill theirs."""
+    import torch
+    full = 128 if hd > 96 else 96 if hd > 64 else 64 if hd > 32 else 32
+    kv = hip.KVCacheF16(1, 8 * full, 8 * full, 40000)
+    for t in kv.tensors(0):
+        t.fill_(NAN)
+    out = torch.empty((n, heads // n_kv * 8 * full), device="cuda")
+    kv.attend_shared_dev(0, torch.ones_like(out), heads // n_kv * 8, 8, full, 0, 40000, None, None, 0, 0.1, out)
+    assert np.isnan(host(out)).all()
+    check_shared(hip, n, heads, n_kv, hd, 2, length, [(length + 9, i % 3) for i in range(n)], length + 20, 355)
+
+
 def test_shared_workspace_is_the_callers(hip):
     import torch
     check_shared(hip, 5, 8, 2, 64, 0, 300, [(300, 20)] * 5, 320, 360, work=True)
