@@ -443,10 +443,11 @@ __device__ __forceinline__ void seq_many(const SeqArgs& a, int b, char* lds) {
             lds_buffer16(w >= kStep * CH / 64 ? v : k, off[u], to + 1024 * w);
         }
     };
-#pragma unroll
-    for (int i = 0; i < kStages - 1; i++) copy(i);
+    copy(0);  // the queries' loads wait for it, not for the stages after
     SeqRows<HD, NQ> q;
     seq_queries<HD, NQ, false>(a, g, 0, row0, p1, q);
+#pragma unroll
+    for (int i = 1; i < kStages - 1; i++) copy(i);
     int lim_all = p1;  // positions that no row of this wave masks
     if (a.causal) lim_all = min(p1, a.start + a.len - (a.n - 1 - min(row0 / a.r, a.n - 1)));
     float minus1 = -1.0f;  // a register, so that w - hi is one mixed-precision fma of hi as it lies
