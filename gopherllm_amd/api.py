@@ -69,35 +69,61 @@ def _host_f32(a, numel: int, what: str):
     return a
 
 
-def _dev_rows(t, kind: str, n: int, dim: int, what: str):
-    """(pointer, row stride) of n rows of at least dim values: a 1-D tensor of
-    one row, or a 2-D tensor whose rows are contiguous and may be apart."""
-    if not getattr(t, "is_cuda", False):
+_kinds = {}
+
+
+def _here():
+    """(current device, its current stream) for the calls that check their
+    tensors' device.  A decode step makes a few such calls per layer, each a few
+    microseconds on the GPU, so they look torch up once and ask it for plain
+    numbers (a torch Stream object alone is 3 us)."""
+    global _torch, _raw_stream
+    if not _kinds:
+        import torch
+        for kind, names in _DTYPES.items():
+            _kinds[kind] = frozenset(getattr(torch, n) for n in names if hasattr(torch, n))
+        _torch = torch
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                              lambda at: torch.cuda.current_stream(at).cuda_stream)
+    at = _torch.cuda.current_device()
+    return at, _raw_stream(at)
+
+
+def _ptr(t, kind: str, numel: int, what: str, at: int):
+    """_dev's pointer of a tensor that has to be on device `at` as well."""
+    if t.dtype in _kinds[kind] and t.get_device() == at and t.numel() >= numel and t.is_contiguous():
+        return t.data_ptr()
+    _dev(t, kind, numel, what)
+    raise ValueError(f"{what}: on device {t.get_device()}, the current one is {at}")
+
+
+def _ptr_rows(t, kind: str, n: int, dim: int, what: str, at: int):
+    """(pointer, row stride) of n rows of dim values: a 1-D tensor of one row, or
+    a 2-D tensor whose rows are contiguous and may be apart."""
+    if t.get_device() < 0:
         raise ValueError(f"{what}: expected a device tensor")
-    if str(t.dtype).replace("torch.", "") not in _DTYPES[kind]:
+    if t.get_device() != at:
+        raise ValueError(f"{what}: on device {t.get_device()}, the current one is {at}")
+    if t.dtype not in _kinds[kind]:
         raise ValueError(f"{what}: dtype {t.dtype}, expected {kind}")
-    if t.dim() == 1:
-        t = t.unsqueeze(0)
-    if t.dim() != 2 or t.shape[0] != n or t.shape[1] < dim:
+    shape = t.shape
+    if len(shape) == 1:
+        shape = (1, shape[0])
+    if len(shape) != 2 or shape[0] != n or shape[1] != dim:
         raise ValueError(f"{what}: shape {tuple(t.shape)}, need {n} rows of {dim}")
-    if t.shape[1] > 1 and t.stride(1) != 1 or n > 1 and t.stride(0) < dim:
-        raise ValueError(f"{what}: the values of a row must be contiguous, and rows must not overlap")
-    return _dev_ptr(t), t.stride(0) if n > 1 else t.shape[1]
+    if not t.is_contiguous():
+        inner, outer = t.stride(-1), t.stride(0) if n > 1 else dim
+        if dim > 1 and inner != 1 or outer < dim:
+            raise ValueError(f"{what}: the values of a row must be contiguous, and rows must not overlap")
+        return t.data_ptr(), outer
+    return t.data_ptr(), dim
 
 
-def _on_current_device(**tensors):
-    import torch
-    at = torch.cuda.current_device()
-    for what, t in tensors.items():
-        if t is not None and t.device.index != at:
-            raise ValueError(f"{what}: on device {t.device.index}, the current one is {at}")
-
-
-def _work(work):
+def _work(work, at):
     """(pointer, bytes) of a caller's workspace, or of none."""
     if work is None:
         return None, 0
-    return _dev(work, "u8", 0, "work"), work.numel()
+    return _ptr(work, "u8", 0, "work", at), work.numel()
 
 
 def _rows(t):
@@ -380,16 +406,16 @@ class Rope:
 
     def apply_dev(self, x, positions, out=None, stream=None):
         """Rotate x (tokens, heads * head_dim) by positions (int32), in place without out."""
+        at, current = _here()
         out = x if out is None else out
-        n = positions.numel()
-        _on_current_device(x=x, positions=positions, out=out)
-        heads = x.shape[-1] // self.head_dim
-        if heads * self.head_dim != x.shape[-1]:
-            raise ValueError(f"x: rows of {x.shape[-1]} are not heads of {self.head_dim}")
-        xp, xs = _dev_rows(x, "f32", n, heads * self.head_dim, "x")
-        op, os = _dev_rows(out, "f32", n, heads * self.head_dim, "out")
-        call("gllm_hip_rope_dev", self.handle, xp, xs, n, heads, _dev(positions, "i32", n, "positions"), op, os,
-             _stream(stream))
+        n, dim = positions.numel(), x.shape[-1]
+        heads = dim // self.head_dim
+        if heads * self.head_dim != dim:
+            raise ValueError(f"x: rows of {dim} are not heads of {self.head_dim}")
+        xp, xs = _ptr_rows(x, "f32", n, dim, "x", at)
+        op, os = _ptr_rows(out, "f32", n, dim, "out", at)
+        call("gllm_hip_rope_dev", self.handle, xp, xs, n, heads, _ptr(positions, "i32", n, "positions", at), op, os,
+             current if stream is None else stream)
         return out
 
     def release(self):
@@ -495,44 +521,49 @@ class KVCacheF16:
         """Rotate q (tokens, heads * hd; or None) into q_out (default: in place) and
         k (tokens, kv heads * hd) by positions, and store k and v as f16 in the
         cache's rows (int32; outside the cache: not stored; all different)."""
+        at, current = _here()
         n, hd = positions.numel(), rope.head_dim
-        q_out = q if q_out is None else q_out
-        _on_current_device(q=q, k=k, v=v, positions=positions, rows=rows, q_out=q_out)
-        heads, n_kv = (0 if q is None else q.shape[-1] // hd), k.shape[-1] // hd
-        if k.shape[-1] != n_kv * hd or v.shape[-1] != k.shape[-1] or q is not None and q.shape[-1] != heads * hd:
-            raise ValueError(f"store_rope_dev: q, k or v rows are not heads of {hd}")
-        qp, qs = (None, 0) if q is None else _dev_rows(q, "f32", n, heads * hd, "q")
-        op, os = (None, 0) if q is None else _dev_rows(q_out, "f32", n, heads * hd, "q_out")
-        kp, ks = _dev_rows(k, "f32", n, n_kv * hd, "k")
-        vp, vs = _dev_rows(v, "f32", n, n_kv * hd, "v")
+        kd, qd = k.shape[-1], 0 if q is None else q.shape[-1]
+        heads, n_kv = qd // hd, kd // hd
+        if kd != n_kv * hd or qd != heads * hd:
+            raise ValueError(f"store_rope_dev: q or k rows are not heads of {hd}")
+        qp = op = None
+        qs = os = 0
+        if q is not None:
+            qp, qs = _ptr_rows(q, "f32", n, qd, "q", at)
+            op, os = (qp, qs) if q_out is None else _ptr_rows(q_out, "f32", n, qd, "q_out", at)
+        kp, ks = _ptr_rows(k, "f32", n, kd, "k", at)
+        vp, vs = _ptr_rows(v, "f32", n, kd, "v", at)
         call("gllm_hip_kv_store_rope_dev", self.handle, layer, rope.handle, qp, qs, heads, kp, ks, vp, vs, n_kv, n,
-             _dev(positions, "i32", n, "positions"), _dev(rows, "i32", n, "rows"), op, os, _stream(stream))
-        return q_out
+             _ptr(positions, "i32", n, "positions", at), _ptr(rows, "i32", n, "rows", at), op, os,
+             current if stream is None else stream)
+        return q if q_out is None else q_out
 
     def attend_shared_dev(self, layer, q, n_heads, n_kv_heads, hd, start, length, starts, lens, most, scale, out,
                           work=None, stream=None):
         """One token of each request: q (requests, n_heads * hd) over the shared rows
         start .. start + length - 1 and, with most > 0, its own lens[i] rows from
         starts[i] (int32 tensors; most: the length the work is split for)."""
+        at, current = _here()
         n = q.shape[0] if q.dim() > 1 else 1
-        _on_current_device(q=q, starts=starts, lens=lens, out=out, work=work)
-        wp, wb = _work(work)
-        call("gllm_hip_attend_shared_dev", self.handle, layer, _dev(q, "f32", n * n_heads * hd, "q"), n, n_heads,
-             n_kv_heads, hd, start, length, None if starts is None else _dev(starts, "i32", n, "starts"),
-             None if lens is None else _dev(lens, "i32", n, "lens"), most, scale,
-             _dev(out, "f32", n * n_heads * hd, "out"), wp, wb, _stream(stream))
+        numel = n * n_heads * hd
+        wp, wb = _work(work, at)
+        call("gllm_hip_attend_shared_dev", self.handle, layer, _ptr(q, "f32", numel, "q", at), n, n_heads, n_kv_heads,
+             hd, start, length, None if starts is None else _ptr(starts, "i32", n, "starts", at),
+             None if lens is None else _ptr(lens, "i32", n, "lens", at), most, scale,
+             _ptr(out, "f32", numel, "out", at), wp, wb, current if stream is None else stream)
         return out
 
     def attend_mass_dev(self, layer, q, n_heads, n_kv_heads, hd, start, end, scale, mass, out, work=None, stream=None):
         """The newest tokens q (tokens, n_heads * hd), the last at row `end`, causally over
         rows start .. end; each row's weight is added to mass (n_kv_heads, >= end + 1)."""
+        at, current = _here()
         n = q.shape[0] if q.dim() > 1 else 1
-        _on_current_device(q=q, mass=mass, out=out, work=work)
-        wp, wb = _work(work)
-        stride = mass.shape[-1]
-        call("gllm_hip_attend_mass_dev", self.handle, layer, _dev(q, "f32", n * n_heads * hd, "q"), n, n_heads,
-             n_kv_heads, hd, start, end, scale, _dev(mass, "f32", n_kv_heads * stride, "mass"), stride,
-             _dev(out, "f32", n * n_heads * hd, "out"), wp, wb, _stream(stream))
+        numel, stride = n * n_heads * hd, mass.shape[-1]
+        wp, wb = _work(work, at)
+        call("gllm_hip_attend_mass_dev", self.handle, layer, _ptr(q, "f32", numel, "q", at), n, n_heads, n_kv_heads, hd,
+             start, end, scale, _ptr(mass, "f32", n_kv_heads * stride, "mass", at), stride,
+             _ptr(out, "f32", numel, "out", at), wp, wb, current if stream is None else stream)
         return out
 
     def keep_dev(self, dst: "KVCacheF16", n_kv_heads, hd, length, budget, mass, pos, mass_out, pos_out, now, sinks=0,
@@ -541,17 +572,17 @@ class KVCacheF16:
         of rows start .. start + length - 1, per layer and kv head, to dst from
         dst_start on.  mass, pos (or None: the row): (layers, n_kv_heads, rows of this
         cache); mass_out, pos_out: (layers, n_kv_heads, rows of dst)."""
-        _on_current_device(mass=mass, pos=pos, mass_out=mass_out, pos_out=pos_out, work=work)
+        at, current = _here()
         stride, out_stride = mass.shape[-1], mass_out.shape[-1]
         if pos is not None and pos.shape[-1] != stride or pos_out.shape[-1] != out_stride:
             raise ValueError("keep_dev: mass and pos rows of different lengths")
         n = self.layers * n_kv_heads
-        wp, wb = _work(work)
+        wp, wb = _work(work, at)
         call("gllm_hip_kv_keep_dev", self.handle, dst.handle, n_kv_heads, hd, start, length, dst_start, budget, sinks,
-             recent, now, _dev(mass, "f32", n * stride, "mass"),
-             None if pos is None else _dev(pos, "i32", n * stride, "pos"), stride,
-             _dev(mass_out, "f32", n * out_stride, "mass_out"), _dev(pos_out, "i32", n * out_stride, "pos_out"),
-             out_stride, wp, wb, _stream(stream))
+             recent, now, _ptr(mass, "f32", n * stride, "mass", at),
+             None if pos is None else _ptr(pos, "i32", n * stride, "pos", at), stride,
+             _ptr(mass_out, "f32", n * out_stride, "mass_out", at), _ptr(pos_out, "i32", n * out_stride, "pos_out", at),
+             out_stride, wp, wb, current if stream is None else stream)
 
     def evict_store_dev(self, layer, n_kv_heads, hd, k, v, start, length, mass, pos, now, sinks=0, recent=0,
                         rows_out=None, stream=None):
@@ -559,12 +590,12 @@ class KVCacheF16:
         unprotected row of least mass among start .. start + length - 1; its pos
         becomes now (an int32 device tensor of one value), its mass 0.  mass, pos:
         (n_kv_heads, rows); rows_out: n_kv_heads int32, the rows given up."""
-        _on_current_device(k=k, v=v, mass=mass, pos=pos, now=now, rows_out=rows_out)
-        stride = mass.shape[-1]
+        at, current = _here()
+        stride, dim = mass.shape[-1], n_kv_heads * hd
         if pos.shape[-1] != stride:
             raise ValueError("evict_store_dev: mass and pos rows of different lengths")
-        call("gllm_hip_kv_evict_store_dev", self.handle, layer, n_kv_heads, hd, _dev(k, "f32", n_kv_heads * hd, "k"),
-             _dev(v, "f32", n_kv_heads * hd, "v"), start, length, sinks, recent,
-             _dev(mass, "f32", n_kv_heads * stride, "mass"), _dev(pos, "i32", n_kv_heads * stride, "pos"), stride,
-             _dev(now, "i32", 1, "now"), None if rows_out is None else _dev(rows_out, "i32", n_kv_heads, "rows_out"),
-             _stream(stream))
+        call("gllm_hip_kv_evict_store_dev", self.handle, layer, n_kv_heads, hd, _ptr(k, "f32", dim, "k", at),
+             _ptr(v, "f32", dim, "v", at), start, length, sinks, recent,
+             _ptr(mass, "f32", n_kv_heads * stride, "mass", at), _ptr(pos, "i32", n_kv_heads * stride, "pos", at), stride,
+             _ptr(now, "i32", 1, "now", at), None if rows_out is None else _ptr(rows_out, "i32", n_kv_heads, "rows_out", at),
+             current if stream is None else stream)

@@ -223,10 +223,3 @@ def test_rope_calls_without_a_rope():
     refused("gllm_hip_rope_dev", g.EINVAL, None, P, 64, 1, 1, P, P, 64, None)
     kv = cache()
     refused("gllm_hip_kv_store_rope_dev", g.EINVAL, C.byref(kv), 0, None, P, 64, 1, P, 64, P, 64, 1, 1, P, P, P, 64, None)
-
-
-def test_python_refuses_host_tensors():
-    import torch
-    t = torch.zeros(4, 64)
-    with pytest.raises(ValueError):
-        g.api._dev_rows(t, "f32", 4, 64, "t")

@@ -440,7 +440,8 @@ def test_rope_no_tokens_and_refusals(hip):
     kv.store_rope_dev(0, rope, none, none, none, ints, ints)
     x, pos = torch.zeros((3, 128), device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
     for bad in (lambda: rope.apply_dev(x[:, :100], pos), lambda: rope.apply_dev(x.double(), pos), lambda: rope.apply_dev(x.T, pos),
-                lambda: rope.apply_dev(x, pos.long()), lambda: rope.apply_dev(x[:2], pos),
+                lambda: rope.apply_dev(x, pos.long()), lambda: rope.apply_dev(x[:2], pos), lambda: rope.apply_dev(x.cpu(), pos),
+                lambda: rope.apply_dev(x, pos.cpu()), lambda: rope.apply_dev(x, pos, x[:1].expand(3, 128)),
                 lambda: kv.store_rope_dev(0, rope, x, x, x[:, :64], pos, pos)):
         with pytest.raises(ValueError):
             bad()
