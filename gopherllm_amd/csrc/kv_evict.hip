@@ -35,77 +35,162 @@ struct KeepArgs {
     long long from;      // now - recent
 };
 
-constexpr int kKeepThreads = 1024;
+constexpr int kKeepThreads = 1024, kKeepWaves = kKeepThreads / 64;
 
-// One workgroup per (layer, kv head): the budget-th largest key by four
-// passes of a byte each, then the kept rows in row order.
+// Sum over the threads after this one, and over all: for counts below 2^31.
+__device__ __forceinline__ int sum_after(int v, int* wave_sums) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int s = v;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int x = __shfl_down(s, off);
+        if (lane + off < 64) s += x;
+    }
+    __syncthreads();  // the sums of an earlier call have been read
+    if (lane == 0) wave_sums[wave] = s;
+    __syncthreads();
+    int after = s - v;
+#pragma unroll
+    for (int w = 0; w < kKeepWaves; w++) after += w > wave ? wave_sums[w] : 0;
+    return after;
+}
+
+// One workgroup per (layer, kv head).  The budget-th largest key by three
+// histograms in LDS of its 12, 10 and 10 leading bits: 12, because weights
+// share their sign and most of their exponent, and an LDS counter that many
+// lanes want serves them one by one (digits of 8 bits took 100 us for 16384
+// rows of 24 layers x 8 heads, counting by ballots, two bits a pass, 52).
+// Then the kept rows in row order, from the counts of every run of 64 rows.
+//
+// KPT: rows of a thread in a tile (row = 1024 (tile KPT + i) + thread); the
+// keys of a single tile stay in registers, those of more are read per pass.
+template <int KPT>
 __global__ __launch_bounds__(kKeepThreads) void keep_select_kernel(KeepArgs a) {
+    constexpr int kTile = KPT * kKeepThreads, kRuns = KPT * kKeepWaves, kBins = 4096;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const size_t lg = blockIdx.x;
     const float* mass = a.mass + lg * a.stride + a.start;
     const int32_t* pos = a.pos ? a.pos + lg * a.stride + a.start : nullptr;
-    __shared__ int hist[256];
-    __shared__ uint32_t s_prefix;
-    __shared__ int s_need;
-    __shared__ int w_gt[kKeepThreads / 64], w_eq[kKeepThreads / 64];
-    const auto key = [&](int t) {
-        const int p = pos ? pos[t] : a.start + t;
-        return kept_always(p, a.sinks, a.from) ? 0xFFFFFFFFu : mass_key(mass[t]);
+    __shared__ __align__(16) int hist[kBins];
+    __shared__ int wave_sums[kKeepWaves], wave_at[kKeepWaves];
+    __shared__ uint32_t s_thr;
+    __shared__ int s_left;
+    uint32_t key[KPT];
+    const auto load = [&](int t0) {
+        float m[KPT];  // all on their way before the first is looked at
+        int p[KPT];
+#pragma unroll
+        for (int i = 0; i < KPT; i++) {
+            const int t = min(t0 + kKeepThreads * i + tid, a.len - 1);
+            m[i] = mass[t];
+            p[i] = a.start + t;
+        }
+        if (pos) {
+#pragma unroll
+            for (int i = 0; i < KPT; i++) p[i] = pos[min(t0 + kKeepThreads * i + tid, a.len - 1)];
+        }
+#pragma unroll
+        for (int i = 0; i < KPT; i++) key[i] = kept_always(p[i], a.sinks, a.from) ? 0xFFFFFFFFu : mass_key(m[i]);
     };
-    uint32_t prefix = 0;
-    int need = a.budget;  // rows still wanted among those with this prefix
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
+    const bool one = a.len <= kTile;
+    if (one) load(0);
+    uint32_t thr = 0;
+    int left = a.budget;  // rows still wanted among the keys with these leading bits
+#pragma unroll
+    for (int pass = 0; pass < 3; pass++) {
+        const int shift = pass == 0 ? 20 : pass == 1 ? 10 : 0, bins = pass == 0 ? kBins : 1024;
+        for (int i = tid; i < bins; i += kKeepThreads) hist[i] = 0;
         __syncthreads();
-        const uint32_t mask = shift == 24 ? 0u : 0xFFFFFFFFu << (shift + 8);
-        for (int t = tid; t < a.len; t += kKeepThreads) {
-            const uint32_t k = key(t);
-            if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
-        }
-        __syncthreads();
-        if (tid == 0) {
-            int b = 255, left = need;
-            while (b > 0 && hist[b] < left) left -= hist[b--];
-            s_prefix = prefix | ((uint32_t)b << shift);
-            s_need = left;
-        }
-        __syncthreads();
-        prefix = s_prefix;
-        need = s_need;
-    }
-    // rows above the threshold, and the first `need` rows at it
-    int done = 0, eq_done = 0;
-    for (int t0 = 0; t0 < a.len; t0 += kKeepThreads) {
-        const int t = t0 + tid;
-        const uint32_t k = t < a.len ? key(t) : 0;
-        const bool eq = t < a.len && k == prefix, gt = t < a.len && k > prefix;
-        const uint64_t be = __ballot(eq), bg = __ballot(gt);
-        if (lane == 0) {
-            w_eq[wave] = __popcll(be);
-            w_gt[wave] = __popcll(bg);
-        }
-        __syncthreads();
-        int eq_before = eq_done, gt_before = 0, eq_all = eq_done, gt_all = 0;
-        for (int w = 0; w < kKeepThreads / 64; w++) {
-            if (w < wave) {
-                eq_before += w_eq[w];
-                gt_before += w_gt[w];
+        for (int t0 = 0; t0 < a.len; t0 += kTile) {
+            if (!one) load(t0);
+#pragma unroll
+            for (int i = 0; i < KPT; i++) {
+                const bool in = pass == 0 || ((key[i] ^ thr) >> (pass == 1 ? 20 : 10)) == 0;
+                if (in && t0 + kKeepThreads * i + tid < a.len) atomicAdd(&hist[(key[i] >> shift) & (bins - 1)], 1);
             }
-            eq_all += w_eq[w];
-            gt_all += w_gt[w];
         }
-        const uint64_t below = (1ull << lane) - 1;
-        eq_before += __popcll(be & below);
-        gt_before += __popcll(bg & below);
-        if (gt || (eq && eq_before < need)) {
-            const int at = done + gt_before + min(eq_before, need) - min(eq_done, need);
-            a.list[lg * a.budget + at] = a.start + t;
-            a.mass_out[lg * a.out_stride + a.dst_start + at] = mass[t];
-            a.pos_out[lg * a.out_stride + a.dst_start + at] = pos ? pos[t] : a.start + t;
-        }
-        done += gt_all + min(eq_all, need) - min(eq_done, need);
-        eq_done = eq_all;
         __syncthreads();
+        // thread t holds the bins 4 t .. 4 t + 3, or t; after: keys in the bins above
+        const int per = bins / kKeepThreads;
+        int c[4] = {0, 0, 0, 0}, mine = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (j < per) mine += c[j] = hist[per * tid + j];
+        int after = sum_after(mine, wave_sums);
+        if (after < left && after + mine >= left) {
+#pragma unroll
+            for (int j = 3; j >= 0; j--) {
+                if (j < per && after < left && after + c[j] >= left) {
+                    s_thr = thr | (uint32_t)(per * tid + j) << shift;
+                    s_left = left - after;
+                    break;
+                }
+                after += c[j];
+            }
+        }
+        __syncthreads();
+        thr = s_thr;
+        left = s_left;
+    }
+    // kept: keys above the threshold, and the first `left` rows at it
+    int* above = hist;  // of each run, then before each run
+    int* at_it = hist + kRuns;
+    static_assert(2 * kRuns <= kBins, "the runs' counts reuse the histogram");
+    int done = 0, at_done = 0;  // rows kept, and keys at the threshold, before this tile
+    for (int t0 = 0; t0 < a.len; t0 += kTile) {
+        if (!one) load(t0);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < KPT; i++) {
+            const bool in = t0 + kKeepThreads * i + tid < a.len;
+            const int up = __popcll(__ballot(in && key[i] > thr)), eq = __popcll(__ballot(in && key[i] == thr));
+            if (lane == 0) {
+                above[i * kKeepWaves + wave] = up;
+                at_it[i * kKeepWaves + wave] = eq;
+            }
+        }
+        __syncthreads();
+        const int u = tid < kRuns ? above[tid] : 0, e = tid < kRuns ? at_it[tid] : 0;
+        int su = u, se = e;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int x = __shfl_up(su, off), y = __shfl_up(se, off);
+            if (lane >= off) {
+                su += x;
+                se += y;
+            }
+        }
+        if (lane == 63) {
+            wave_sums[wave] = su;
+            wave_at[wave] = se;
+        }
+        __syncthreads();
+        int bu = 0, be = 0, up_all = 0, at_all = 0;
+        for (int w = 0; w < kKeepWaves; w++) {
+            bu += w < wave ? wave_sums[w] : 0;
+            be += w < wave ? wave_at[w] : 0;
+            up_all += wave_sums[w];
+            at_all += wave_at[w];
+        }
+        if (tid < kRuns) {
+            above[tid] = bu + su - u;
+            at_it[tid] = be + se - e;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < KPT; i++) {
+            const int t = t0 + kKeepThreads * i + tid;
+            const bool gt = t < a.len && key[i] > thr, eq = t < a.len && key[i] == thr;
+            const uint64_t below = (1ull << lane) - 1;
+            const int up = above[i * kKeepWaves + wave] + __popcll(__ballot(gt) & below);
+            const int before = at_done + at_it[i * kKeepWaves + wave] + __popcll(__ballot(eq) & below);
+            if (gt || (eq && before < left)) {
+                const int at = done + up + min(before, left) - min(at_done, left);
+                a.list[lg * a.budget + at] = a.start + t;  // the copy brings its mass and position
+            }
+        }
+        done += up_all + min(at_done + at_all, left) - min(at_done, left);
+        at_done += at_all;
     }
 }
 
@@ -115,18 +200,24 @@ struct KeepPtrs {
     uint16_t *dk[kKeepLayers], *dv[kKeepLayers];
 };
 
-// dst row dst_start + j of head g = src row list[j]; 16 bytes a thread.
-__global__ __launch_bounds__(256) void keep_copy_kernel(KeepPtrs p, const int32_t* __restrict__ list, int layer0, int n_kv,
-                                                        int hd, int budget, int dst_start, int sk, int sv, int dk, int dv) {
+// dst row dst_start + j of head g = src row list[j], with its mass and
+// position; 16 bytes a thread.
+__global__ __launch_bounds__(256) void keep_copy_kernel(KeepPtrs p, KeepArgs a, int layer0, int hd, int sk, int sv, int dk,
+                                                        int dv) {
     const int l = blockIdx.y, ch = hd / 8;
     const long long e = (long long)blockIdx.x * 256 + threadIdx.x;  // (row, head, chunk)
-    if (e >= (long long)budget * n_kv * ch) return;
-    const int c = (int)(e % ch), g = (int)(e / ch % n_kv), j = (int)(e / ch / n_kv);
-    const size_t row = list[((size_t)(layer0 + l) * n_kv + g) * budget + j], to = (size_t)dst_start + j;
+    if (e >= (long long)a.budget * a.n_kv * ch) return;
+    const int c = (int)(e % ch), g = (int)(e / ch % a.n_kv), j = (int)(e / ch / a.n_kv);
+    const size_t lg = (size_t)(layer0 + l) * a.n_kv + g;
+    const size_t row = a.list[lg * a.budget + j], to = (size_t)a.dst_start + j;
     const int col = g * hd + 8 * c;
     const u4 kk = *(const u4*)(p.k[l] + row * sk + col), vv = *(const u4*)(p.v[l] + row * sv + col);
     *(u4*)(p.dk[l] + to * dk + col) = kk;
     *(u4*)(p.dv[l] + to * dv + col) = vv;
+    if (c == 0) {
+        a.mass_out[lg * a.out_stride + to] = a.mass[lg * a.stride + row];
+        a.pos_out[lg * a.out_stride + to] = a.pos ? a.pos[lg * a.stride + row] : (int)row;
+    }
 }
 
 struct EvictArgs {
@@ -151,13 +242,13 @@ __global__ __launch_bounds__(kKeepThreads) void evict_store_kernel(EvictArgs a) 
         const uint32_t k = kept_always(pos[t], a.sinks, from) ? 0xFFFFFFFFu : mass_key(mass[t]);
         best = min(best, (uint64_t)k << 32 | (uint32_t)t);
     }
-    __shared__ uint64_t wb[kKeepThreads / 64];
+    __shared__ uint64_t wb[kKeepWaves];
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) best = min(best, (uint64_t)__shfl_xor((unsigned long long)best, off));
     if ((tid & 63) == 0) wb[tid >> 6] = best;
     __syncthreads();
     best = wb[0];
-    for (int w = 1; w < kKeepThreads / 64; w++) best = min(best, wb[w]);
+    for (int w = 1; w < kKeepWaves; w++) best = min(best, wb[w]);
     const int t = (int)(uint32_t)best;
     const size_t row = (size_t)a.start + t;
     if (tid < a.hd) {
@@ -226,7 +317,9 @@ int gllm_hip_kv_keep_dev(const gllm_hip_kv* src, gllm_hip_kv* dst, int n_kv_head
     if (!list) return scratch_error();
     KeepArgs a{d_mass, d_pos, d_mass_out, d_pos_out, list, n_kv_heads, stride, out_stride, start, dst_start, len, budget, sinks,
                (long long)now - recent};
-    hipLaunchKernelGGL(keep_select_kernel, dim3((unsigned)(src->layers * n_kv_heads)), dim3(kKeepThreads), 0, s, a);
+    const dim3 grid((unsigned)(src->layers * n_kv_heads)), block(kKeepThreads);
+    if (len <= 4 * kKeepThreads) hipLaunchKernelGGL(keep_select_kernel<4>, grid, block, 0, s, a);
+    else hipLaunchKernelGGL(keep_select_kernel<16>, grid, block, 0, s, a);
     GLLM_HIP(hipGetLastError());
     const long long items = (long long)budget * n_kv_heads * (hd / 8);
     for (int l0 = 0; l0 < src->layers; l0 += kKeepLayers) {
@@ -238,8 +331,8 @@ int gllm_hip_kv_keep_dev(const gllm_hip_kv* src, gllm_hip_kv* dst, int n_kv_head
             p.dk[i] = dst->k[l0 + i];
             p.dv[i] = dst->v[l0 + i];
         }
-        hipLaunchKernelGGL(keep_copy_kernel, dim3((unsigned)((items + 255) / 256), (unsigned)n), dim3(256), 0, s, p, list, l0,
-                           n_kv_heads, hd, budget, dst_start, src->kv_dim_k, src->kv_dim_v, dst->kv_dim_k, dst->kv_dim_v);
+        hipLaunchKernelGGL(keep_copy_kernel, dim3((unsigned)((items + 255) / 256), (unsigned)n), dim3(256), 0, s, p, a, l0, hd,
+                           src->kv_dim_k, src->kv_dim_v, dst->kv_dim_k, dst->kv_dim_v);
         GLLM_HIP(hipGetLastError());
     }
     return GLLM_OK;

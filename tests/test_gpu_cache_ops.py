@@ -475,6 +475,8 @@ def masses(seed, shape):
 @pytest.mark.parametrize("layers,n_kv,hd,start,length,dst_start,budget,sinks,recent,with_pos", [
     (1, 1, 8, 0, 1, 0, 1, 0, 0, False), (2, 2, 64, 3, 50, 2, 20, 4, 5, True), (1, 8, 128, 0, 1025, 0, 300, 0, 0, False),
     (3, 3, 40, 1, 2500, 0, 2500, 4, 100, True), (1, 2, 32, 0, 700, 5, 1, 2, 3, True), (1, 1, 16, 0, 5000, 0, 4999, 0, 64, False),
+    (1, 1, 8, 0, 4096, 0, 700, 4, 9, True), (1, 2, 8, 0, 16385, 0, 9000, 4, 9, True), (1, 1, 8, 3, 65536, 0, 30000, 0, 100, False),
+    (1, 2, 8, 0, 65537, 0, 20000, 4, 64, True), (1, 1, 8, 0, 140001, 1, 139000, 4, 64, True), (1, 1, 8, 0, 100000, 0, 1, 0, 0, True),
     (40, 1, 8, 0, 90, 0, 30, 1, 9, True), (1, 2, 64, 0, 300, 0, 50, 100, 100, True), (1, 2, 64, 0, 6000, 0, 1000, 0, 0, True),
 ])
 def test_keep(hip, layers, n_kv, hd, start, length, dst_start, budget, sinks, recent, with_pos):
