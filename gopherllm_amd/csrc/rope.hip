@@ -65,18 +65,111 @@ struct RopeArgs {
     const int32_t* rows;  // cache rows, null: q alone
     uint16_t *K, *V;
     int kd_k, kd_v, max_len;
+    uint64_t unit_magic;  // ceil(2^32 / units of a head)
 };
 
-// One workgroup per token.
-__global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
-    __shared__ float2 cs[512];
-    const size_t t = blockIdx.x;
-    const int half = a.rot / 2;
-    for (int i = threadIdx.x; i < half; i += 256) {
+// cos and sin of a token's angles, times the amplitude, into cs
+__device__ __forceinline__ void rope_angles(const RopeArgs& a, int t, float2* cs) {
+    for (int i = threadIdx.x; i < a.rot / 2; i += 256) {
         double s, c;
         sincos64((double)a.pos[t] * a.inv[i], &s, &c);
         cs[i] = make_float2((float)(c * a.amp), (float)(s * a.amp));
     }
+}
+
+__device__ __forceinline__ float2 turn(float x0, float x1, float2 w) {
+    return make_float2(fmaf(x0, w.x, -(x1 * w.y)), fmaf(x0, w.y, x1 * w.x));
+}
+
+// The row that unit e of a token is in
+__device__ __forceinline__ const float* rope_source(const RopeArgs& a, size_t t, int e, int n_q, int n_k) {
+    const bool is_q = e < n_q, is_k = e < n_q + n_k;
+    const size_t stride = is_q ? a.q_stride : is_k ? a.k_stride : a.v_stride;
+    const uintptr_t base = is_q ? (uintptr_t)a.q : is_k ? (uintptr_t)a.k : (uintptr_t)a.v;
+    return (const float*)base + t * stride;
+}
+
+// A token's queries, keys and values in units of four values (HALF: of two
+// such quads half a rotation apart), one a thread; blockIdx.y takes the
+// units from its number times 256 on, in steps of the grid, and its first
+// unit is on its way while the angles are made.  Bound by memory: 4001 tokens
+// of 32 / 8 heads of 128 (180 MB) took 54 us one value a thread.
+template <bool HALF>
+__global__ __launch_bounds__(256) void rope_quads_kernel(RopeArgs a) {
+    __shared__ __align__(16) float2 cs[512];
+    const size_t t = blockIdx.x;
+    const int half = a.rot / 2;
+    const int row = a.rows ? a.rows[t] : -1;
+    const bool store = row >= 0 && row < a.max_len;
+    const int unit = (HALF ? a.hd - half : a.hd) / 4;  // of a head
+    const int n_q = a.q ? a.heads * unit : 0, n_k = store ? a.n_kv * unit : 0, n_v = store ? a.n_kv * a.hd / 4 : 0;
+    const int all = n_q + n_k + n_v, step = 256 * gridDim.y;
+    const float4 none = make_float4(0, 0, 0, 0);
+    // unit e: its head's unit u (past the head's turning values for v), and its place in the row of heads
+    const auto place = [&](int e, int& u) {
+        if (e >= n_q + n_k) {
+            u = a.hd;
+            return 4 * (e - n_q - n_k);
+        }
+        const int f = e < n_q ? e : e - n_q, h = (int)(((uint64_t)f * a.unit_magic) >> 32);  // f / unit
+        u = f - h * unit;
+        return h * a.hd + 4 * u + (HALF && 4 * u >= half ? half : 0);
+    };
+    const auto finish = [&](int e, int u, int at, float4 x, float4 y) {
+        const bool two = HALF && 4 * u < half;
+        if (two) {
+            const float4 w0 = *(const float4*)&cs[4 * u], w1 = *(const float4*)&cs[4 * u + 2];
+            const float2 p0 = turn(x.x, y.x, make_float2(w0.x, w0.y)), p1 = turn(x.y, y.y, make_float2(w0.z, w0.w));
+            const float2 p2 = turn(x.z, y.z, make_float2(w1.x, w1.y)), p3 = turn(x.w, y.w, make_float2(w1.z, w1.w));
+            x = make_float4(p0.x, p1.x, p2.x, p3.x);
+            y = make_float4(p0.y, p1.y, p2.y, p3.y);
+        } else if (!HALF && 4 * u < a.rot) {
+            const float4 w = *(const float4*)&cs[2 * u];
+            const float2 p0 = turn(x.x, x.y, make_float2(w.x, w.y)), p1 = turn(x.z, x.w, make_float2(w.z, w.w));
+            x = make_float4(p0.x, p0.y, p1.x, p1.y);
+        }
+        if (e < n_q) {
+            float* o = a.q_out + t * a.out_stride + at;
+            *(float4*)o = x;
+            if (two) *(float4*)(o + half) = y;
+        } else {
+            const auto pack = [](float4 f) {
+                return make_uint2(f32_to_f16_bits(f.x) | (uint32_t)f32_to_f16_bits(f.y) << 16,
+                                  f32_to_f16_bits(f.z) | (uint32_t)f32_to_f16_bits(f.w) << 16);
+            };
+            uint16_t* o = (e < n_q + n_k ? a.K + (size_t)row * a.kd_k : a.V + (size_t)row * a.kd_v) + at;
+            *(uint2*)o = pack(x);
+            if (two) *(uint2*)(o + half) = pack(y);
+        }
+    };
+    int e = blockIdx.y * 256 + threadIdx.x, u = 0, at = 0;
+    float4 x = none, y = none;
+    if (e < all) {
+        at = place(e, u);
+        const float* src = rope_source(a, t, e, n_q, n_k) + at;
+        x = *(const float4*)src;
+        if (HALF && 4 * u < half) y = *(const float4*)(src + half);
+    }
+    rope_angles(a, t, cs);
+    __syncthreads();
+    if (e < all) finish(e, u, at, x, y);
+    for (e += step; e < all; e += step) {
+        at = place(e, u);
+        const float* src = rope_source(a, t, e, n_q, n_k) + at;
+        x = *(const float4*)src;
+        y = none;
+        if (HALF && 4 * u < half) y = *(const float4*)(src + half);
+        finish(e, u, at, x, y);
+    }
+}
+
+// The same for any sizes and alignments, a pair or a value that stays at a
+// time.  One workgroup per token.
+__global__ __launch_bounds__(256) void rope_pairs_kernel(RopeArgs a) {
+    __shared__ float2 cs[512];
+    const size_t t = blockIdx.x;
+    const int half = a.rot / 2;
+    rope_angles(a, t, cs);
     __syncthreads();
     const int row = a.rows ? a.rows[t] : -1;
     const bool store = row >= 0 && row < a.max_len;
@@ -87,26 +180,23 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
         const int f = is_q ? e : e - n_q, h = f / unit, i = f - h * unit;
         const float* x = (is_q ? a.q + t * a.q_stride : a.k + t * a.k_stride) + h * a.hd;
         int i0, i1;
-        float y0, y1;
+        float2 y;
         if (i < half) {
             i0 = a.half_layout ? i : 2 * i;
             i1 = a.half_layout ? i + half : 2 * i + 1;
-            const float x0 = x[i0], x1 = x[i1];
-            const float2 w = cs[i];
-            y0 = fmaf(x0, w.x, -(x1 * w.y));
-            y1 = fmaf(x0, w.y, x1 * w.x);
+            y = turn(x[i0], x[i1], cs[i]);
         } else {
             i0 = i1 = i + half;
-            y0 = y1 = x[i0];
+            y.x = y.y = x[i0];
         }
         if (is_q) {
             float* o = a.q_out + t * a.out_stride + h * a.hd;
-            o[i0] = y0;
-            o[i1] = y1;
+            o[i0] = y.x;
+            o[i1] = y.y;
         } else {
             uint16_t* o = a.K + (size_t)row * a.kd_k + h * a.hd;
-            o[i0] = f32_to_f16_bits(y0);
-            o[i1] = f32_to_f16_bits(y1);
+            o[i0] = f32_to_f16_bits(y.x);
+            o[i1] = f32_to_f16_bits(y.y);
         }
     }
     if (store)
@@ -114,9 +204,25 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
             a.V[(size_t)row * a.kd_v + e] = f32_to_f16_bits(a.v[t * a.v_stride + e]);
 }
 
-static int rope_launch(const RopeArgs& a, int n, hipStream_t s) {
+static int rope_launch(RopeArgs a, int n, hipStream_t s) {
     if (n == 0) return GLLM_OK;
-    hipLaunchKernelGGL(rope_kernel, dim3((unsigned)n), dim3(256), 0, s, a);
+    // quads: 16-byte loads and 8-byte f16 stores, and no quad that turns in part
+    const uintptr_t ptrs = (uintptr_t)a.q | (uintptr_t)a.q_out | (uintptr_t)a.k | (uintptr_t)a.v;
+    const int strides = (a.q ? a.q_stride | a.out_stride : 0) | (a.rows ? a.k_stride | a.v_stride | a.kd_k | a.kd_v : 0);
+    if (ptrs % 16 == 0 && strides % 4 == 0 && a.hd % 4 == 0 && a.rot % (a.half_layout ? 8 : 4) == 0) {
+        const int unit = (a.half_layout ? a.hd - a.rot / 2 : a.hd) / 4;
+        const long long all = (a.q ? (long long)a.heads * unit : 0) + (a.rows ? (long long)a.n_kv * (unit + a.hd / 4) : 0);
+        if (all < 65536) {  // where the multiplication divides exactly
+            a.unit_magic = (0x100000000ull + unit - 1) / unit;
+            // a few tokens: their units over several workgroups
+            const int parts = std::max(1, std::min((int)((all + 255) / 256), 512 / n));
+            if (a.half_layout) hipLaunchKernelGGL(rope_quads_kernel<true>, dim3((unsigned)n, parts), dim3(256), 0, s, a);
+            else hipLaunchKernelGGL(rope_quads_kernel<false>, dim3((unsigned)n, parts), dim3(256), 0, s, a);
+            GLLM_HIP(hipGetLastError());
+            return GLLM_OK;
+        }
+    }
+    hipLaunchKernelGGL(rope_pairs_kernel, dim3((unsigned)n), dim3(256), 0, s, a);
     GLLM_HIP(hipGetLastError());
     return GLLM_OK;
 }
