@@ -51,14 +51,34 @@ inline SeqPlan seq_plan(int n, int n_heads, int n_kv, int len, int most) {
     return p;
 }
 
-// Floats of the workspace: base and sum of every partial result, its output,
-// and for `scored` positions the scores of every row with the row's final
-// base and 1 / sum.
-inline size_t seq_floats(const SeqPlan& p, int hd, size_t scored) {
-    const size_t parts = p.rows * (size_t)p.slots;
-    size_t f = parts * (2 + (size_t)hd);
-    return f + p.rows * scored + 64;
+// Floats of the partial results: base and sum of each, and its output.
+inline size_t seq_floats(const SeqPlan& p, int hd) { return p.rows * (size_t)p.slots * (2 + (size_t)hd) + 64; }
+
+// What attention with weights works in, in floats: few query rows a kv head keep
+// their scores, many keep their operands (f16 pairs, in the matrix cores' order),
+// scales and final base and 1 / sum; then the partial results.
+struct MassSpace {
+    bool kept;
+    int sstride;  // of a row's scores
+    int tiles;    // of 16 query rows of a kv head
+    size_t scale, ml, parts;
+};
+inline MassSpace mass_space(const SeqPlan& p, int hd, int n_kv, int len) {
+    MassSpace m{};
+    m.kept = p.rw == 1;
+    if (m.kept) {
+        m.sstride = (int)(((size_t)len + 3) / 4 * 4);
+        m.parts = p.rows * (size_t)m.sstride;
+    } else {
+        m.tiles = p.row_blocks * p.rw * p.nq;
+        const size_t all = (size_t)m.tiles * n_kv;
+        m.scale = all * 2 * ceil_div(hd, 32) * 64 * 4;  // 16 bytes a lane for each 32 dims of both parts
+        m.ml = m.scale + all * 16;
+        m.parts = m.ml + (p.rows * 2 + 3) / 4 * 4;
+    }
+    return m;
 }
+inline size_t mass_floats(const SeqPlan& p, int hd, int n_kv, int len) { return mass_space(p, hd, n_kv, len).parts + seq_floats(p, hd); }
 
 // Rows a .. b - 1 of a cache of max_len rows that the range start, len names.
 struct RowSpan {

@@ -53,8 +53,11 @@ struct SeqArgs {
     float* pm;            // [row][slot] base
     float* pl;            //             sum
     float* po;            //             [hd] output
-    float* scores;        // [row][sstride] or null
+    float* scores;        // few rows: [row][sstride], or null
     int sstride;
+    u4* q_parts;          // many rows: the queries' operands [kv head][tile of 16 rows][lo, hi][32 dims][lane], or null
+    float* q_scale;       // [kv head][tile][16]: score of a dot of theirs, in powers of two
+    int tiles;            // of a kv head
 };
 
 // A new base puts the largest weight so far at 2^8; it stays until a weight
@@ -448,6 +451,18 @@ __device__ __forceinline__ void seq_many(const SeqArgs& a, int b, char* lds) {
     seq_queries<HD, NQ, false>(a, g, 0, row0, p1, q);
 #pragma unroll
     for (int i = 1; i < kStages - 1; i++) copy(i);
+    if (a.q_parts && slot == 0) {
+#pragma unroll
+        for (int nq = 0; nq < NQ; nq++) {
+            const size_t tile = (size_t)g * a.tiles + row0 / 16 + nq;
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++) {
+                a.q_parts[(tile * 2 * KK + kk) * 64 + lane] = __builtin_bit_cast(u4, q.lo[nq][kk]);
+                a.q_parts[(tile * 2 * KK + KK + kk) * 64 + lane] = __builtin_bit_cast(u4, q.hi[nq][kk]);
+            }
+            if (grp == 0) a.q_scale[tile * 16 + col] = q.c[nq];
+        }
+    }
     int lim_all = p1;  // positions that no row of this wave masks
     if (a.causal) lim_all = min(p1, a.start + a.len - (a.n - 1 - min(row0 / a.r, a.n - 1)));
     float minus1 = -1.0f;  // a register, so that w - hi is one mixed-precision fma of hi as it lies
@@ -471,7 +486,7 @@ __device__ __forceinline__ void seq_many(const SeqArgs& a, int b, char* lds) {
             seq_dot<HD, NQ>(k, q, s, t);
         }
         const int pb = p0 + it * kStep;
-        seq_step<HD, NQ>(a, g, row0, pb, p1, pb + kStep <= lim_all, a.scores != nullptr, s, q, kt + TILE, minus1);
+        seq_step<HD, NQ>(a, g, row0, pb, p1, pb + kStep <= lim_all, false, s, q, kt + TILE, minus1);
     }
     wait_vmem_le<0>();  // no copy outlives the workgroup
 #pragma unroll
@@ -525,29 +540,32 @@ __device__ __forceinline__ SlotFactors slot_factors(const float* pm, const float
 struct MergeArgs {
     const float *pm, *pl, *po;
     float* out;
+    float2* ml;           // base and 1 / sum of each row, or null
     int rows, slots, hd;
-    const float* scores;  // [row][sstride], or null: no mass
+    const float* scores;  // few rows: [row][sstride], or null
     float* mass;          // [kv head][mass_stride], from the first attended row on
     int sstride, n, n_heads, n_kv, r, len, mass_stride, mass_wgs;
 };
 
-constexpr int kMassRows = 64;  // query rows whose base and 1 / sum a workgroup holds at a time
+constexpr int kFewRows = 16;         // query rows of a kv head up to which scores are kept
+constexpr int kMassPositions = 512;  // of a workgroup
 
-// Workgroups below mass_wgs add the weights of 512 positions to mass, the
-// others make a row's output:
+// Workgroups below mass_wgs add the weights of 512 positions to mass, from the
+// kept scores of a kv head's few query rows; the others make a row's output:
 // out[row] = sum_s 2^(base_s - M) o_s / sum_s 2^(base_s - M) l_s, zero for a row
 // without positions; 32 threads take a slot, 4 dims each, eight slots at a time.
 __global__ __launch_bounds__(256) void seq_merge_kernel(MergeArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    __shared__ __align__(16) float red[8][128];
     if ((int)blockIdx.x >= a.mass_wgs) {
+        __shared__ __align__(16) float red[8][128];
+        __shared__ float f[2 * kSeqMaxSplits];
         const size_t row = blockIdx.x - a.mass_wgs, at = row * a.slots;
         const SlotFactors s = slot_factors(a.pm, a.pl, at, a.slots, lane);
         const float inv = s.L == 0.0f ? 0.0f : 1.0f / s.L;
-        __shared__ float f[2 * kSeqMaxSplits];
         if (wave == 0) {
             f[lane] = s.f0;
             f[lane + 64] = s.f1;
+            if (a.ml && lane == 0) a.ml[row] = make_float2(s.L == 0.0f ? 0.0f : s.M, inv);
         }
         __syncthreads();
         const int sub = tid >> 5, d = 4 * (tid & 31);
@@ -567,34 +585,111 @@ __global__ __launch_bounds__(256) void seq_merge_kernel(MergeArgs a) {
         }
         return;
     }
-    __shared__ float2 ml[kMassRows];  // base, 1 / sum
-    const int g = blockIdx.x % a.n_kv, t = (blockIdx.x / a.n_kv) * 512 + 2 * tid;
+    __shared__ float2 ml[kFewRows];
+    const int g = blockIdx.x % a.n_kv, t = (blockIdx.x / a.n_kv) * kMassPositions + 2 * tid;
     const int rows = a.n * a.r;
+    const auto row_of = [&](int q) { return (size_t)(q / a.r) * a.n_heads + g * a.r + q % a.r; };
+    for (int q = wave; q < rows; q += 4) {
+        const SlotFactors s = slot_factors(a.pm, a.pl, row_of(q) * a.slots, a.slots, lane);
+        if (lane == 0) ml[q] = make_float2(s.L == 0.0f ? 0.0f : s.M, s.L == 0.0f ? 0.0f : 1.0f / s.L);
+    }
+    __syncthreads();
     float s0 = 0.0f, s1 = 0.0f;
-    for (int r0 = 0; r0 < rows; r0 += kMassRows) {
-        const int m = min(kMassRows, rows - r0);
-        __syncthreads();
-        for (int q = wave; q < m; q += 4) {
-            const int i = (r0 + q) / a.r;
-            const size_t row = (size_t)i * a.n_heads + g * a.r + (r0 + q - i * a.r);
-            const SlotFactors s = slot_factors(a.pm, a.pl, row * a.slots, a.slots, lane);
-            if (lane == 0) ml[q] = make_float2(s.L == 0.0f ? 0.0f : s.M, s.L == 0.0f ? 0.0f : 1.0f / s.L);
-        }
-        __syncthreads();
-        if (t < a.len) {
+    if (t < a.len) {
 #pragma unroll 8
-            for (int q = 0; q < m; q++) {
-                const int i = (r0 + q) / a.r;
-                const size_t row = (size_t)i * a.n_heads + g * a.r + (r0 + q - i * a.r);
-                const float2 x = *(const float2*)(a.scores + row * a.sstride + t), b = ml[q];
-                s0 = fmaf(__builtin_amdgcn_exp2f(x.x - b.x), b.y, s0);
-                s1 = fmaf(__builtin_amdgcn_exp2f(x.y - b.x), b.y, s1);
-            }
+        for (int q = 0; q < rows; q++) {
+            const float2 x = *(const float2*)(a.scores + row_of(q) * a.sstride + t), b = ml[q];
+            s0 = fmaf(__builtin_amdgcn_exp2f(x.x - b.x), b.y, s0);
+            s1 = fmaf(__builtin_amdgcn_exp2f(x.y - b.x), b.y, s1);
         }
     }
     float* to = a.mass + (size_t)g * a.mass_stride + t;
     if (t < a.len) to[0] += s0;
     if (t + 1 < a.len) to[1] += s1;
+}
+
+struct MassArgs {
+    const uint16_t* K;
+    const u4* q_parts;
+    const float* q_scale;
+    const float2* ml;
+    float* mass;  // from the first attended row on
+    int kd_k, hd, n, n_heads, n_kv, r, tiles, start, len, mass_stride;
+};
+
+// The weights of many query rows, from their scores made again: a wave holds 64
+// positions' keys in registers and takes the rows' operands, 16 rows at a time,
+// as the attention left them.  Reading K twice (33 MB for 16001 rows of 8 heads
+// of 128) costs less than writing and reading the scores of 32 tokens (65 MB each
+// way: 44 + 40 us for both kernels).
+template <int HD>
+__global__ __launch_bounds__(256, 2) void seq_mass_kernel(MassArgs a) {
+    constexpr int KK = HD / 32, PT = 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, grp = lane >> 4;
+    const int g = blockIdx.x % a.n_kv, p0 = (blockIdx.x / a.n_kv) * 256 + wave * 64;
+    if (p0 >= a.len) return;
+    h8 k[PT][KK];
+#pragma unroll
+    for (int t = 0; t < PT; t += 2) {
+        const SeqBuffer b(a.K, a.kd_k, a.hd, g, a.start + min(p0 + 16 * t, a.len), a.start + a.len);
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++) {
+                const int d = 32 * kk + 8 * grp;
+                k[t + u][kk] = __builtin_bit_cast(h8, b.load(d < a.hd ? ((16 * u + col) * a.kd_k + d) * 2 : kPastEnd));
+            }
+    }
+    f4 sum[PT];
+#pragma unroll
+    for (int t = 0; t < PT; t++) sum[t] = f4{0, 0, 0, 0};
+    const u4* parts = a.q_parts + (size_t)g * a.tiles * 2 * KK * 64 + lane;
+    const int rows = a.n * a.r, tiles = (rows + 15) / 16;
+    u4 next[2 * KK];
+#pragma unroll
+    for (int i = 0; i < 2 * KK; i++) next[i] = parts[i * 64];
+    for (int tile = 0; tile < tiles; tile++) {
+        h8 q[2 * KK];
+#pragma unroll
+        for (int i = 0; i < 2 * KK; i++) q[i] = __builtin_bit_cast(h8, next[i]);
+        const int rr = 16 * tile + col, i = min(rr, rows - 1) / a.r;
+        const float2 b = a.ml[(size_t)i * a.n_heads + g * a.r + (min(rr, rows - 1) - i * a.r)];
+        const float c = a.q_scale[((size_t)g * a.tiles + tile) * 16 + col], inv = rr < rows ? b.y : 0.0f;
+        const int lim = a.len - (a.n - 1 - i);  // positions from it on are masked
+        if (tile + 1 < tiles) {
+#pragma unroll
+            for (int j = 0; j < 2 * KK; j++) next[j] = parts[((tile + 1) * 2 * KK + j) * 64];
+        }
+        f4 s[PT];
+#pragma unroll
+        for (int t = 0; t < PT; t++) s[t] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) {
+#pragma unroll
+            for (int t = 0; t < PT; t++) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][kk], q[kk], s[t], 0, 0, 0);
+#pragma unroll
+            for (int t = 0; t < PT; t++) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][kk], q[KK + kk], s[t], 0, 0, 0);
+        }
+#pragma unroll
+        for (int t = 0; t < PT; t++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float w = __builtin_amdgcn_exp2f(fmaf(s[t][j], c, -b.x)) * inv;
+                sum[t][j] += p0 + 16 * t + 4 * grp + j < lim ? w : 0.0f;
+            }
+    }
+    // over the 16 rows of the tiles; position 16 t + 4 grp + j
+#pragma unroll
+    for (int t = 0; t < PT; t++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float x = sum[t][j];
+#pragma unroll
+            for (int off = 8; off >= 1; off >>= 1) x += __shfl_xor(x, off);
+            const int p = p0 + 16 * t + 4 * grp + j;
+            if (col == 0 && p < a.len) a.mass[(size_t)g * a.mass_stride + p] += x;
+        }
 }
 
 template <int NQ, int RW>
@@ -702,7 +797,7 @@ size_t gllm_hip_attend_shared_bytes(int n, int n_heads, int n_kv_heads, int hd, 
     if (n < 1 || n_kv_heads < 1 || n_heads < 1 || n_heads % n_kv_heads || hd < 1 || len < 0 || most < 0 ||
         (long long)n * n_heads > (1 << 24))
         return 0;
-    return 4 * seq_floats(seq_plan(n, n_heads, n_kv_heads, len, most), hd, 0);
+    return 4 * seq_floats(seq_plan(n, n_heads, n_kv_heads, len, most), hd);
 }
 
 int gllm_hip_attend_shared_dev(gllm_hip_kv* kv, int l, const float* d_q, int n, int n_heads, int n_kv_heads, int hd,
@@ -717,7 +812,7 @@ int gllm_hip_attend_shared_dev(gllm_hip_kv* kv, int l, const float* d_q, int n, 
     hipStream_t s = (hipStream_t)stream;
     const SeqPlan p = seq_plan(n, n_heads, n_kv_heads, len, most);
     float* w;
-    GLLM_TRY(seq_work(what, kv, seq_floats(p, hd, 0), d_work, work_bytes, s, &w));
+    GLLM_TRY(seq_work(what, kv, seq_floats(p, hd), d_work, work_bytes, s, &w));
     SeqArgs a = seq_args(kv, l, d_q, n, n_heads, n_kv_heads, hd, scale, p, w);
     a.start = start;
     a.len = len;
@@ -730,10 +825,10 @@ int gllm_hip_attend_shared_dev(gllm_hip_kv* kv, int l, const float* d_q, int n, 
 }
 
 size_t gllm_hip_attend_mass_bytes(int n, int n_heads, int n_kv_heads, int hd, int len) {
-    if (n < 1 || n_kv_heads < 1 || n_heads < 1 || n_heads % n_kv_heads || hd < 1 || len < 1 ||
+    if (n < 1 || n_kv_heads < 1 || n_heads < 1 || n_heads % n_kv_heads || hd < 1 || hd > 128 || len < 1 ||
         (long long)n * n_heads > (1 << 24))
         return 0;
-    return 4 * seq_floats(seq_plan(n, n_heads, n_kv_heads, len, 0), hd, ((size_t)len + 3) / 4 * 4);
+    return 4 * mass_floats(seq_plan(n, n_heads, n_kv_heads, len, 0), hd, n_kv_heads, len);
 }
 
 int gllm_hip_attend_mass_dev(gllm_hip_kv* kv, int l, const float* d_q, int n, int n_heads, int n_kv_heads, int hd,
@@ -746,25 +841,44 @@ int gllm_hip_attend_mass_dev(gllm_hip_kv* kv, int l, const float* d_q, int n, in
     if (!d_mass || mass_stride <= end) return fail(GLLM_EINVAL, "%s: mass rows of %d values do not hold position %d", what, mass_stride, end);
     hipStream_t s = (hipStream_t)stream;
     const int len = end - start + 1;
-    const int sstride = (int)(((size_t)len + 3) / 4 * 4);
     const SeqPlan p = seq_plan(n, n_heads, n_kv_heads, len, 0);
     float* w;
-    GLLM_TRY(seq_work(what, kv, seq_floats(p, hd, sstride), d_work, work_bytes, s, &w));
-    SeqArgs a = seq_args(kv, l, d_q, n, n_heads, n_kv_heads, hd, scale, p, w + p.rows * (size_t)sstride);
+    GLLM_TRY(seq_work(what, kv, mass_floats(p, hd, n_kv_heads, len), d_work, work_bytes, s, &w));
+    const MassSpace m = mass_space(p, hd, n_kv_heads, len);
+    SeqArgs a = seq_args(kv, l, d_q, n, n_heads, n_kv_heads, hd, scale, p, w + m.parts);
     a.start = start;
     a.len = len;
     a.causal = 1;
-    a.scores = w;
-    a.sstride = sstride;
+    if (m.kept) {
+        a.scores = w;
+        a.sstride = m.sstride;
+    } else {
+        a.q_parts = (u4*)w;
+        a.q_scale = w + m.scale;
+        a.tiles = m.tiles;
+    }
     GLLM_TRY(seq_launch(a, p, s));
-    MergeArgs m = merge_args(a, p, d_out);
-    m.scores = w;
-    m.sstride = sstride;
-    m.mass = d_mass + start;
-    m.mass_stride = mass_stride;
-    m.mass_wgs = n_kv_heads * ((len + 511) / 512);
-    hipLaunchKernelGGL(seq_merge_kernel, dim3((unsigned)(m.mass_wgs + p.rows)), dim3(256), 0, s, m);
+    MergeArgs g = merge_args(a, p, d_out);
+    g.mass = d_mass + start;
+    g.mass_stride = mass_stride;
+    if (m.kept) {
+        g.scores = w;
+        g.sstride = m.sstride;
+        g.mass_wgs = n_kv_heads * ((len + kMassPositions - 1) / kMassPositions);
+    } else {
+        g.ml = (float2*)(w + m.ml);
+    }
+    hipLaunchKernelGGL(seq_merge_kernel, dim3((unsigned)(g.mass_wgs + p.rows)), dim3(256), 0, s, g);
     GLLM_HIP(hipGetLastError());
+    if (!m.kept) {
+        const MassArgs b{a.K, a.q_parts, a.q_scale, g.ml, g.mass, a.kd_k, hd, n, n_heads, n_kv_heads, p.r, m.tiles, start, len, mass_stride};
+        const dim3 grid((unsigned)(n_kv_heads * ((len + 255) / 256)));
+        if (hd <= 32) hipLaunchKernelGGL(seq_mass_kernel<32>, grid, dim3(256), 0, s, b);
+        else if (hd <= 64) hipLaunchKernelGGL(seq_mass_kernel<64>, grid, dim3(256), 0, s, b);
+        else if (hd <= 96) hipLaunchKernelGGL(seq_mass_kernel<96>, grid, dim3(256), 0, s, b);
+        else hipLaunchKernelGGL(seq_mass_kernel<128>, grid, dim3(256), 0, s, b);
+        GLLM_HIP(hipGetLastError());
+    }
     return GLLM_OK;
 }
 

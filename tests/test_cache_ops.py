@@ -40,8 +40,18 @@ int main() {
             need((long long)p.chunk * p.chunks >= len && (long long)p.chunk * (p.chunks - 1) < len, "cover", n, h, g, len, most);
         }
         if (most) need(p.own_blocks * 16 >= r, "own blocks", n, h, g, len, most);
-        need(seq_floats(p, 128, 0) >= p.rows * (size_t)p.slots * 130, "floats", n, h, g, len, most);
-        need(seq_floats(p, 128, 64) >= p.rows * (size_t)p.slots * 130 + p.rows * 64, "scored", n, h, g, len, most);
+        need(seq_floats(p, 128) >= p.rows * (size_t)p.slots * 130, "floats", n, h, g, len, most);
+        if (len && !most)
+            for (int hd : {8, 40, 96, 128}) {
+                const MassSpace m = mass_space(p, hd, g, len);
+                const int kk = hd <= 32 ? 1 : hd <= 64 ? 2 : hd <= 96 ? 3 : 4;
+                need(m.kept == (n * r <= 16), "kept", n, h, g, len, hd);
+                need(m.parts % 4 == 0 && m.scale % 4 == 0 && m.ml % 4 == 0, "aligned", n, h, g, len, hd);
+                if (m.kept) need(m.sstride >= len && m.sstride % 4 == 0 && m.parts == p.rows * (size_t)m.sstride, "scores", n, h, g, len, hd);
+                else need(16LL * m.tiles >= (long long)n * r && m.scale == (size_t)g * m.tiles * 2 * kk * 64 * 4 &&
+                          m.ml >= m.scale + (size_t)g * m.tiles * 16 && m.parts >= m.ml + 2 * p.rows, "operands", n, h, g, len, hd);
+                need(mass_floats(p, hd, g, len) >= m.parts + p.rows * (size_t)p.slots * (2 + hd), "mass floats", n, h, g, len, hd);
+            }
     }
     const int big = 2147483647;
     struct { int s, l, m, a, b; } cut[] = {{0, 5, 10, 0, 5}, {7, 5, 10, 7, 10}, {-3, 5, 10, 0, 2}, {-9, 5, 10, 0, 0}, {12, 5, 10, 10, 10},
@@ -177,7 +187,7 @@ def test_attend_needs_aligned_rows_and_32_bit_rows():
 
 def test_workspace_sizes():
     assert g.attend_shared_bytes(0, 8, 2, 64, 1, 0) == 0 and g.attend_shared_bytes(1, 8, 3, 64, 1, 0) == 0
-    assert g.attend_shared_bytes(4, 8, 2, 64, 100, 9) > 0 and g.attend_mass_bytes(4, 8, 2, 64, 100) > 4 * 8 * 100 * 4
+    assert g.attend_shared_bytes(4, 8, 2, 64, 100, 9) > 0 and g.attend_mass_bytes(4, 8, 2, 64, 100) > 4 * 8 * 100 * 4 and g.attend_mass_bytes(1, 8, 2, 129, 100) == 0
     assert g.attend_mass_bytes(1, 8, 2, 64, 0) == 0
     assert g.keep_bytes(3, 2, 5) == 120 and g.keep_bytes(0, 2, 5) == 0
 
