@@ -37,7 +37,12 @@ inline SeqPlan seq_plan(int n, int n_heads, int n_kv, int len, int most) {
     p.row_blocks = (int)((per_kv + 16 * p.nq * p.rw - 1) / (16 * p.nq * p.rw));
     if (len > 0) {
         const long long per_chunk = (long long)n_kv * p.row_blocks;
-        const int want = (int)std::max(1LL, std::min((long long)kSeqMaxSplits, kSeqTarget / per_chunk));
+        // Many rows of a shared range keep the matrix cores busy and the own
+        // ranges memory: where these are as long, half the workgroups leave room
+        // for both on a CU (64 requests over 32768 rows and up to 1024 of their
+        // own: 120 us with 512, 114 with 256; without own ranges 78 and 89).
+        const int target = p.rw > 1 && (long long)n * most >= len ? kSeqTarget / 2 : kSeqTarget;
+        const int want = (int)std::max(1LL, std::min((long long)kSeqMaxSplits, target / per_chunk));
         p.chunk = ceil_div(ceil_div(len, want), kSeqQuantum) * kSeqQuantum;
         p.chunks = ceil_div(len, p.chunk);
     }
