@@ -12,6 +12,7 @@ constexpr int kSeqWaves = 4;                  // waves of a workgroup
 constexpr int kSeqQuantum = 128;              // positions: one step of every shape of workgroup, or more
 constexpr int kSeqTarget = 512;               // workgroups: two for each of the 256 CUs
 constexpr int kSeqMaxSplits = 64;             // partial results of a query row from one range
+constexpr int kSeqMaxRows = 1 << 22;          // n * n_heads: a workgroup each has to fit a launch
 
 // Query rows of a kv head: n tokens x r heads.
 struct SeqPlan {
@@ -59,8 +60,8 @@ inline SeqPlan seq_plan(int n, int n_heads, int n_kv, int len, int most) {
 // Floats of the partial results: base and sum of each, and its output.
 inline size_t seq_floats(const SeqPlan& p, int hd) { return p.rows * (size_t)p.slots * (2 + (size_t)hd) + 64; }
 
-// What attention with weights works in, in floats: few query rows a kv head keep
-// their scores, many keep their operands (f16 pairs, in the matrix cores' order),
+// What attention with weights works in, in floats: one token's query rows (up to
+// 16 a kv head) keep their scores, more keep their operands (f16 pairs, in the matrix cores' order),
 // scales and final base and 1 / sum; then the partial results.
 struct MassSpace {
     bool kept;
@@ -70,7 +71,7 @@ struct MassSpace {
 };
 inline MassSpace mass_space(const SeqPlan& p, int hd, int n_kv, int len) {
     MassSpace m{};
-    m.kept = p.rw == 1;
+    m.kept = p.rw == 1 && p.rows == (size_t)n_kv * p.r;
     if (m.kept) {
         m.sstride = (int)(((size_t)len + 3) / 4 * 4);
         m.parts = p.rows * (size_t)m.sstride;

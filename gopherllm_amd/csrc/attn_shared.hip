@@ -42,10 +42,10 @@ struct SeqArgs {
     int kd_k, kd_v;       // row strides
     int n, n_heads, n_kv, r, hd, max_len;
     int start, len;       // shared rows
-    int causal;           // token i ends n - 1 - i rows earlier
     int row_blocks, chunk;
-    const int32_t* starts;  // own rows
+    const int32_t* starts;  // own rows, or null: token i has the i rows from own_row on
     const int32_t* lens;
+    int own_row;
     int own_blocks, splits;
     int shared_wgs;       // workgroups of the shared range
     int slot0, slots;     // first partial of the own ranges, partials per row
@@ -53,9 +53,9 @@ struct SeqArgs {
     float* pm;            // [row][slot] base
     float* pl;            //             sum
     float* po;            //             [hd] output
-    float* scores;        // few rows: [row][sstride], or null
+    float* scores;        // one token: [row][sstride], or null
     int sstride;
-    u4* q_parts;          // many rows: the queries' operands [kv head][tile of 16 rows][lo, hi][32 dims][lane], or null
+    u4* q_parts;          // more: the queries' operands [kv head][tile of 16 rows][lo, hi][32 dims][lane], or null
     float* q_scale;       // [kv head][tile][16]: score of a dot of theirs, in powers of two
     int tiles;            // of a kv head
 };
@@ -96,14 +96,13 @@ template <int HD, int NQ>
 struct SeqRows {
     h8 hi[NQ][HD / 32], lo[NQ][HD / 32];
     float c[NQ];
-    int lim[NQ];  // cache rows from it on are masked
     // and the sums so far: out^T tiles of 16 dims, base and sum of weights of this lane's positions
     f4 o[NQ][HD / 16];
     float base[NQ], l[NQ];
 };
 
 template <int HD, int NQ, bool OWN>
-__device__ __forceinline__ void seq_queries(const SeqArgs& a, int g, int tok, int row0, int p1, SeqRows<HD, NQ>& q) {
+__device__ __forceinline__ void seq_queries(const SeqArgs& a, int g, int tok, int row0, SeqRows<HD, NQ>& q) {
     constexpr int KK = HD / 32;
     const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
     const int rows = OWN ? a.r : a.n * a.r;
@@ -113,7 +112,6 @@ __device__ __forceinline__ void seq_queries(const SeqArgs& a, int g, int tok, in
         const bool on = rr < rows;
         const int i = OWN ? tok : rr / a.r, hh = OWN ? rr : rr - i * a.r;
         const size_t row = on ? (size_t)i * a.n_heads + g * a.r + hh : 0;
-        q.lim[nq] = a.causal ? min(p1, a.start + a.len - (a.n - 1 - (on ? i : 0))) : p1;
         f4 x[KK][2];
         float mx = 0.0f;
 #pragma unroll
@@ -151,6 +149,23 @@ __device__ __forceinline__ void seq_queries(const SeqArgs& a, int g, int tok, in
     }
 }
 
+// The operands of the query rows from row0 on, for seq_mass_kernel
+template <int HD, int NQ>
+__device__ __forceinline__ void seq_keep_queries(const SeqArgs& a, int g, int row0, const SeqRows<HD, NQ>& q) {
+    constexpr int KK = HD / 32;
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int nq = 0; nq < NQ; nq++) {
+        const size_t tile = (size_t)g * a.tiles + row0 / 16 + nq;
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) {
+            a.q_parts[(tile * 2 * KK + kk) * 64 + lane] = __builtin_bit_cast(u4, q.lo[nq][kk]);
+            a.q_parts[(tile * 2 * KK + KK + kk) * 64 + lane] = __builtin_bit_cast(u4, q.hi[nq][kk]);
+        }
+        if (lane < 16) a.q_scale[tile * 16 + lane] = q.c[nq];
+    }
+}
+
 // s[nq][t] += K rows (16 positions of tile t) times the query rows
 template <int HD, int NQ>
 __device__ __forceinline__ void seq_dot(const h8 (&k)[HD / 32], const SeqRows<HD, NQ>& q, f4 (&s)[NQ][2], int t) {
@@ -165,26 +180,26 @@ __device__ __forceinline__ void seq_dot(const h8 (&k)[HD / 32], const SeqRows<HD
     }
 }
 
-// The step at position pb: scores s to weights, and the weighted rows of the V
-// tile at vt (LDS) added to the sums.  open: nothing in the step is masked.
+// The step at position pb of a range that ends at p1: scores s to weights, and
+// the weighted rows of the V tile at vt (LDS) added to the sums.
 template <int HD, int NQ>
-__device__ __forceinline__ void seq_step(const SeqArgs& a, int g, int row0, int pb, int p1, bool open, bool scored,
-                                         f4 (&s)[NQ][2], SeqRows<HD, NQ>& q, const char* vt, float minus1) {
+__device__ __forceinline__ void seq_step(const SeqArgs& a, int g, int row0, int pb, int p1, bool scored, f4 (&s)[NQ][2],
+                                         SeqRows<HD, NQ>& q, const char* vt, float minus1) {
     constexpr int DT = HD / 16;
     const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
     const float ninf = -__int_as_float(0x7f800000);
-    // where the step holds masked positions, scaled scores with -Inf in their places
+    // in the range's last step, scaled scores with -Inf past its end
     float cc[NQ];
 #pragma unroll
     for (int nq = 0; nq < NQ; nq++) cc[nq] = q.c[nq];
-    if (!open) {
+    if (pb + kStep > p1) {
 #pragma unroll
         for (int nq = 0; nq < NQ; nq++) {
             cc[nq] = 1.0f;
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) s[nq][t][j] = pb + 16 * t + 4 * grp + j < q.lim[nq] ? s[nq][t][j] * q.c[nq] : ninf;
+                for (int j = 0; j < 4; j++) s[nq][t][j] = pb + 16 * t + 4 * grp + j < p1 ? s[nq][t][j] * q.c[nq] : ninf;
         }
     }
     if (scored) {
@@ -310,7 +325,7 @@ __device__ __forceinline__ void seq_few(const SeqArgs& a, int b, char* lds, floa
         b /= a.own_blocks;
         tok = b % a.n;
         slot = b / a.n;
-        const RowSpan s = clip_rows(a.starts[tok], a.lens[tok], a.max_len);
+        const RowSpan s = a.starts ? clip_rows(a.starts[tok], a.lens[tok], a.max_len) : RowSpan{a.own_row, a.own_row + tok};
         const int chunk = (((s.b - s.a) + a.splits - 1) / a.splits + kSeqQuantum - 1) / kSeqQuantum * kSeqQuantum;
         a0 = min(s.b, s.a + slot * chunk);
         a1 = min(s.b, a0 + chunk);
@@ -348,9 +363,8 @@ __device__ __forceinline__ void seq_few(const SeqArgs& a, int b, char* lds, floa
         load_k(p0);
     }
     SeqRows<HD, 1> q;
-    seq_queries<HD, 1, OWN>(a, g, tok, row0, p1, q);
-    int lim_all = p1;  // positions that no row of this wave masks
-    if (!OWN && a.causal) lim_all = min(p1, a.start + a.len - (a.n - 1 - row0 / a.r));
+    seq_queries<HD, 1, OWN>(a, g, tok, row0, q);
+    if (!OWN && a.q_parts && slot == 0 && wave == 0) seq_keep_queries<HD, 1>(a, g, row0, q);
     float minus1 = -1.0f;  // a register, so that w - hi is one mixed-precision fma of hi as it lies
     asm volatile("" : "+v"(minus1));
     char* vt = lds + wave * SeqLds<HD, 1>::TILE;
@@ -371,7 +385,7 @@ __device__ __forceinline__ void seq_few(const SeqArgs& a, int b, char* lds, floa
             seq_dot<HD, 1>(k, q, s, t);
         }
         if (more) load_k(pb + kStep);
-        seq_step<HD, 1>(a, g, row0, pb, p1, pb + kStep <= lim_all, !OWN && a.scores, s, q, vt, minus1);
+        seq_step<HD, 1>(a, g, row0, pb, p1, !OWN && a.scores, s, q, vt, minus1);
         asm volatile("" ::: "memory");
     }
 
@@ -448,23 +462,10 @@ __device__ __forceinline__ void seq_many(const SeqArgs& a, int b, char* lds) {
     };
     copy(0);  // the queries' loads wait for it, not for the stages after
     SeqRows<HD, NQ> q;
-    seq_queries<HD, NQ, false>(a, g, 0, row0, p1, q);
+    seq_queries<HD, NQ, false>(a, g, 0, row0, q);
 #pragma unroll
     for (int i = 1; i < kStages - 1; i++) copy(i);
-    if (a.q_parts && slot == 0) {
-#pragma unroll
-        for (int nq = 0; nq < NQ; nq++) {
-            const size_t tile = (size_t)g * a.tiles + row0 / 16 + nq;
-#pragma unroll
-            for (int kk = 0; kk < KK; kk++) {
-                a.q_parts[(tile * 2 * KK + kk) * 64 + lane] = __builtin_bit_cast(u4, q.lo[nq][kk]);
-                a.q_parts[(tile * 2 * KK + KK + kk) * 64 + lane] = __builtin_bit_cast(u4, q.hi[nq][kk]);
-            }
-            if (grp == 0) a.q_scale[tile * 16 + col] = q.c[nq];
-        }
-    }
-    int lim_all = p1;  // positions that no row of this wave masks
-    if (a.causal) lim_all = min(p1, a.start + a.len - (a.n - 1 - min(row0 / a.r, a.n - 1)));
+    if (a.q_parts && slot == 0) seq_keep_queries<HD, NQ>(a, g, row0, q);
     float minus1 = -1.0f;  // a register, so that w - hi is one mixed-precision fma of hi as it lies
     asm volatile("" : "+v"(minus1));
     const int steps = (p1 - p0 + kStep - 1) / kStep;
@@ -486,7 +487,7 @@ __device__ __forceinline__ void seq_many(const SeqArgs& a, int b, char* lds) {
             seq_dot<HD, NQ>(k, q, s, t);
         }
         const int pb = p0 + it * kStep;
-        seq_step<HD, NQ>(a, g, row0, pb, p1, pb + kStep <= lim_all, false, s, q, kt + TILE, minus1);
+        seq_step<HD, NQ>(a, g, row0, pb, p1, false, s, q, kt + TILE, minus1);
     }
     wait_vmem_le<0>();  // no copy outlives the workgroup
 #pragma unroll
@@ -542,7 +543,7 @@ struct MergeArgs {
     float* out;
     float2* ml;           // base and 1 / sum of each row, or null
     int rows, slots, hd;
-    const float* scores;  // few rows: [row][sstride], or null
+    const float* scores;  // one token: [row][sstride], or null
     float* mass;          // [kv head][mass_stride], from the first attended row on
     int sstride, n, n_heads, n_kv, r, len, mass_stride, mass_wgs;
 };
@@ -551,7 +552,7 @@ constexpr int kFewRows = 16;         // query rows of a kv head up to which scor
 constexpr int kMassPositions = 512;  // of a workgroup
 
 // Workgroups below mass_wgs add the weights of 512 positions to mass, from the
-// kept scores of a kv head's few query rows; the others make a row's output:
+// kept scores of one token's up to 16 query rows a kv head; the others make a row's output:
 // out[row] = sum_s 2^(base_s - M) o_s / sum_s 2^(base_s - M) l_s, zero for a row
 // without positions; 32 threads take a slot, 4 dims each, eight slots at a time.
 __global__ __launch_bounds__(256) void seq_merge_kernel(MergeArgs a) {
@@ -617,7 +618,7 @@ struct MassArgs {
     int kd_k, hd, n, n_heads, n_kv, r, tiles, start, len, mass_stride;
 };
 
-// The weights of many query rows, from their scores made again: a wave holds 64
+// The weights of several tokens, from their scores made again: a wave holds 64
 // positions' keys in registers and takes the rows' operands, 16 rows at a time,
 // as the attention left them.  Reading K twice (33 MB for 16001 rows of 8 heads
 // of 128) costs less than writing and reading the scores of 32 tokens (65 MB each
@@ -705,12 +706,13 @@ static int seq_check(const char* what, const gllm_hip_kv* kv, int l, const float
     if (n < 1) return fail(GLLM_EINVAL, "%s: %d tokens", what, n);
     if (n_kv < 1 || n_heads < 1 || n_heads % n_kv) return fail(GLLM_EINVAL, "%s: %d heads over %d kv heads", what, n_heads, n_kv);
     if (hd < 8 || hd % 8 || hd > 128) return fail(GLLM_EINVAL, "%s: head size %d is not a multiple of 8 up to 128", what, hd);
-    if ((long long)n * n_heads > (1 << 24)) return fail(GLLM_EINVAL, "%s: %d tokens of %d heads are too many", what, n, n_heads);
+    if ((long long)n * n_heads > kSeqMaxRows) return fail(GLLM_EINVAL, "%s: %d tokens of %d heads are too many", what, n, n_heads);
     if (!kv || !d_q || !d_out) return fail(GLLM_EINVAL, "%s: null pointer", what);
     if (l < 0 || l >= kv->layers) return fail(GLLM_EINVAL, "%s: layer %d out of range", what, l);
     if ((long long)n_kv * hd > kv->kv_dim_k || (long long)n_kv * hd > kv->kv_dim_v)
         return fail(GLLM_EINVAL, "%s: %d kv heads of %d do not fit the cache", what, n_kv, hd);
-    if (kv->max_len > 1 << 30) return fail(GLLM_EUNSUP, "%s: a cache of %d rows", what, kv->max_len);
+    if (kv->max_len > 1 << 30 || kv->kv_dim_k > 1 << 24 || kv->kv_dim_v > 1 << 24)
+        return fail(GLLM_EUNSUP, "%s: a cache of %d rows of %d and %d values", what, kv->max_len, kv->kv_dim_k, kv->kv_dim_v);
     if (kv->kv_dim_k % 8 || kv->kv_dim_v % 8)
         return fail(GLLM_EUNSUP, "%s: cache rows of %d and %d values are not 16-byte aligned", what, kv->kv_dim_k, kv->kv_dim_v);
     if (((uintptr_t)d_q | (uintptr_t)d_out) & 15) return fail(GLLM_EINVAL, "%s: q and out must be 16-byte aligned", what);
@@ -794,8 +796,8 @@ using namespace gllm;
 extern "C" {
 
 size_t gllm_hip_attend_shared_bytes(int n, int n_heads, int n_kv_heads, int hd, int len, int most) {
-    if (n < 1 || n_kv_heads < 1 || n_heads < 1 || n_heads % n_kv_heads || hd < 1 || len < 0 || most < 0 ||
-        (long long)n * n_heads > (1 << 24))
+    if (n < 1 || n_kv_heads < 1 || n_heads < 1 || n_heads % n_kv_heads || hd < 1 || hd > 128 || len < 0 || most < 0 ||
+        (long long)n * n_heads > kSeqMaxRows)
         return 0;
     return 4 * seq_floats(seq_plan(n, n_heads, n_kv_heads, len, most), hd);
 }
@@ -826,9 +828,9 @@ int gllm_hip_attend_shared_dev(gllm_hip_kv* kv, int l, const float* d_q, int n, 
 
 size_t gllm_hip_attend_mass_bytes(int n, int n_heads, int n_kv_heads, int hd, int len) {
     if (n < 1 || n_kv_heads < 1 || n_heads < 1 || n_heads % n_kv_heads || hd < 1 || hd > 128 || len < 1 ||
-        (long long)n * n_heads > (1 << 24))
+        n > len || (long long)n * n_heads > kSeqMaxRows)
         return 0;
-    return 4 * mass_floats(seq_plan(n, n_heads, n_kv_heads, len, 0), hd, n_kv_heads, len);
+    return 4 * mass_floats(seq_plan(n, n_heads, n_kv_heads, len - (n - 1), n - 1), hd, n_kv_heads, len);
 }
 
 int gllm_hip_attend_mass_dev(gllm_hip_kv* kv, int l, const float* d_q, int n, int n_heads, int n_kv_heads, int hd,
@@ -841,14 +843,15 @@ int gllm_hip_attend_mass_dev(gllm_hip_kv* kv, int l, const float* d_q, int n, in
     if (!d_mass || mass_stride <= end) return fail(GLLM_EINVAL, "%s: mass rows of %d values do not hold position %d", what, mass_stride, end);
     hipStream_t s = (hipStream_t)stream;
     const int len = end - start + 1;
-    const SeqPlan p = seq_plan(n, n_heads, n_kv_heads, len, 0);
+    // what every token attends is the shared range; token i has i rows more
+    const SeqPlan p = seq_plan(n, n_heads, n_kv_heads, len - (n - 1), n - 1);
     float* w;
     GLLM_TRY(seq_work(what, kv, mass_floats(p, hd, n_kv_heads, len), d_work, work_bytes, s, &w));
     const MassSpace m = mass_space(p, hd, n_kv_heads, len);
     SeqArgs a = seq_args(kv, l, d_q, n, n_heads, n_kv_heads, hd, scale, p, w + m.parts);
     a.start = start;
-    a.len = len;
-    a.causal = 1;
+    a.len = len - (n - 1);
+    a.own_row = start + a.len;
     if (m.kept) {
         a.scores = w;
         a.sstride = m.sstride;
@@ -859,6 +862,7 @@ int gllm_hip_attend_mass_dev(gllm_hip_kv* kv, int l, const float* d_q, int n, in
     }
     GLLM_TRY(seq_launch(a, p, s));
     MergeArgs g = merge_args(a, p, d_out);
+    g.len = len;
     g.mass = d_mass + start;
     g.mass_stride = mass_stride;
     if (m.kept) {

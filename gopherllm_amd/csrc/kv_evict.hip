@@ -311,6 +311,8 @@ int gllm_hip_kv_keep_dev(const gllm_hip_kv* src, gllm_hip_kv* dst, int n_kv_head
         return fail(GLLM_EUNSUP, "%s: cache rows are not 16-byte aligned", what);
     if (start < 0 || (long long)start + len > src->max_len || dst_start < 0 || (long long)dst_start + budget > dst->max_len)
         return fail(GLLM_EINVAL, "%s: rows %d + %d of %d, to %d + %d of %d", what, start, len, src->max_len, dst_start, budget, dst->max_len);
+    if (src->max_len > 1 << 30 || dst->max_len > 1 << 30 || budget * dim / 8 >= 1LL << 31)
+        return fail(GLLM_EUNSUP, "%s: %d rows of %lld values from %d", what, budget, dim, src->max_len);
     if (stride < start + len || out_stride < dst_start + budget)
         return fail(GLLM_EINVAL, "%s: mass rows of %d and %d values do not hold the rows", what, stride, out_stride);
     const size_t heads = (size_t)src->layers * n_kv_heads;
@@ -364,6 +366,7 @@ int gllm_hip_kv_evict_store_dev(gllm_hip_kv* kv, int l, int n_kv_heads, int hd, 
         return fail(GLLM_EINVAL, "%s: %d kv heads of %d do not fit the cache", what, n_kv_heads, hd);
     if (start < 0 || (long long)start + len > kv->max_len || stride < start + len)
         return fail(GLLM_EINVAL, "%s: rows %d + %d of %d, mass rows of %d", what, start, len, kv->max_len, stride);
+    if (kv->max_len > 1 << 30) return fail(GLLM_EUNSUP, "%s: a cache of %d rows", what, kv->max_len);
     GLLM_TRY(current_is(what, kv));
     EvictArgs a{d_k, d_v, d_mass, d_pos, d_now, d_rows_out, kv->k[l], kv->v[l], stride, start, len, sinks, recent, hd,
                 kv->kv_dim_k, kv->kv_dim_v};

@@ -29,8 +29,8 @@ namespace gllm {
 // Sine and cosine of a by reduction to [-pi/4, pi/4]: a - n pi/2 with pi/2 in
 // two parts, each step one fma, then the Taylor series through r^13 and r^12
 // (the first terms left out are below 2e-14 and 4e-13, a float32 rounding is
-// 6e-8).  Exact to float32 for |a| < 2^31: n needs 31 bits and the products'
-// rounding is absorbed by the fma.
+// 6e-8).  |a| < 2^41 (an int32 position times an inverse frequency below 2^10):
+// n pi/2 loses nothing that a itself, rounded once to 64 bits, still has.
 __device__ __forceinline__ void sincos64(double a, double* s, double* c) {
     const double n = rint(a * 0.63661977236758134308);
     double r = fma(-n, 1.57079632679489655800, a);
@@ -230,6 +230,7 @@ static int rope_launch(RopeArgs a, int n, hipStream_t s) {
 static int rope_check(const char* what, const gllm_hip_rope* r, int n, const int32_t* d_pos) {
     if (!r) return fail(GLLM_EINVAL, "%s: null rope", what);
     if (n < 0 || (n > 0 && !d_pos)) return fail(GLLM_EINVAL, "%s: %d tokens without positions", what, n);
+    if (n >= 1 << 24) return fail(GLLM_EINVAL, "%s: %d tokens are more than a launch holds", what, n);
     int dev = -1;
     GLLM_HIP(hipGetDevice(&dev));
     if (dev != r->device) return fail(GLLM_EINVAL, "%s: the rope is on device %d, the current one is %d", what, r->device, dev);

@@ -68,7 +68,7 @@ inline const char* rope_config_error(const gllm_hip_rope_config& c) {
     }
     if (c.freq_factors)
         for (int i = 0; i < c.rot_dim / 2; i++)
-            if (!pos(c.freq_factors[i])) return "freq_factors must be finite and > 0";
+            if (!(pos(c.freq_factors[i]) && c.freq_factors[i] >= 1e-3f)) return "freq_factors must be finite and >= 0.001";
     return nullptr;
 }
 

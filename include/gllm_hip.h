@@ -295,7 +295,7 @@ typedef struct gllm_hip_rope_config {
     int head_dim, rot_dim; /* the first rot_dim (even) values of a head turn, the others stay */
     int layout, scaling;
     int orig_ctx;
-    const float* freq_factors; /* null, or rot_dim / 2 divisors (rope_freqs.weight) */
+    const float* freq_factors; /* null, or rot_dim / 2 divisors >= 0.001 (rope_freqs.weight) */
     double theta, factor, low_freq_factor, high_freq_factor, beta_fast, beta_slow;
     double attn_factor; /* amplitude of the rotated values; yarn multiplies it by 0.1 ln(factor) + 1 */
 } gllm_hip_rope_config;
@@ -309,8 +309,8 @@ gllm_hip_rope* gllm_hip_rope_new(const gllm_hip_rope_config* cfg);
 void gllm_hip_rope_release(gllm_hip_rope* r);
 /* Rotate the heads of n tokens: d_x and d_out are rows of heads * head_dim
  * floats, x_stride and out_stride apart; token t turns by d_pos[t].  d_out may
- * be d_x (with the same stride) and must not overlap it otherwise.  Angles are
- * 64-bit products, right to float32 for every int32 position. */
+ * be d_x (with the same stride) and must not overlap it otherwise.  The angle
+ * is a 64-bit product, its sine and cosine are rounded to float32 once. */
 int gllm_hip_rope_dev(const gllm_hip_rope* r, const float* d_x, int x_stride, int n, int heads,
                       const int32_t* d_pos, float* d_out, int out_stride, void* stream);
 /* The same for the queries and keys of n tokens, with the store: rotated keys
@@ -334,8 +334,9 @@ int gllm_hip_kv_store_rope_dev(gllm_hip_kv* kv, int l, const gllm_hip_rope* r, c
  * states.  Ranges may overlap: several tokens of one request are several
  * requests whose own ranges start together (a row in both ranges counts
  * twice).  A request without any row gets zeros.  Sums are float32, products
- * of 22-bit q and weights; where an attended row holds an infinity or NaN the
- * outputs of its kv head are not finite. */
+ * of 22-bit q and weights.  Rows outside a request's ranges may hold anything;
+ * where an attended row holds an infinity or NaN the outputs of its kv head are
+ * not defined. */
 size_t gllm_hip_attend_shared_bytes(int n, int n_heads, int n_kv_heads, int hd, int len, int most);
 int gllm_hip_attend_shared_dev(gllm_hip_kv* kv, int l, const float* d_q, int n, int n_heads,
                                int n_kv_heads, int hd, int start, int len,

@@ -45,7 +45,7 @@ int main() {
             for (int hd : {8, 40, 96, 128}) {
                 const MassSpace m = mass_space(p, hd, g, len);
                 const int kk = hd <= 32 ? 1 : hd <= 64 ? 2 : hd <= 96 ? 3 : 4;
-                need(m.kept == (n * r <= 16), "kept", n, h, g, len, hd);
+                need(m.kept == (n == 1 && r <= 16), "kept", n, h, g, len, hd);
                 need(m.parts % 4 == 0 && m.scale % 4 == 0 && m.ml % 4 == 0, "aligned", n, h, g, len, hd);
                 if (m.kept) need(m.sstride >= len && m.sstride % 4 == 0 && m.parts == p.rows * (size_t)m.sstride, "scores", n, h, g, len, hd);
                 else need(16LL * m.tiles >= (long long)n * r && m.scale == (size_t)g * m.tiles * 2 * kk * 64 * 4 &&
@@ -115,7 +115,7 @@ def test_yarn_frequencies():
     dict(theta=float("nan")), dict(theta=-5.0), dict(scaling="linear", factor=0.5), dict(scaling="linear", factor=float("inf")),
     dict(scaling="yarn", factor=2.0), dict(scaling="yarn", factor=2.0, orig_ctx=100, beta_fast=1.0, beta_slow=2.0),
     dict(scaling="llama3", factor=2.0, orig_ctx=100, low_freq_factor=4.0, high_freq_factor=4.0), dict(attn_factor=0.0),
-    dict(freq_factors=np.zeros(64, np.float32)), dict(freq_factors=np.full(64, np.nan, np.float32))])
+    dict(freq_factors=np.zeros(64, np.float32)), dict(freq_factors=np.full(64, 1e-20, np.float32)), dict(freq_factors=np.full(64, np.nan, np.float32))])
 def test_rope_refusals(kw):
     args = dict(head_dim=128)
     args.update(kw)
@@ -180,7 +180,7 @@ def test_attend_mass_refusals(kw):
 
 
 def test_attend_needs_aligned_rows_and_32_bit_rows():
-    for kv in (cache(kd=260), cache(vd=257), cache(rows=(1 << 30) + 1)):
+    for kv in (cache(kd=260), cache(vd=257), cache(rows=(1 << 30) + 1), cache(kd=(1 << 24) + 8)):
         refused("gllm_hip_attend_shared_dev", g.EUNSUP, *dict(SHARED, kv=C.byref(kv)).values())
         refused("gllm_hip_attend_mass_dev", g.EUNSUP, *dict(MASS, kv=C.byref(kv)).values())
 
@@ -213,6 +213,12 @@ def test_keep_refuses_itself_other_layers_and_unaligned_rows():
     refused("gllm_hip_kv_keep_dev", g.EINVAL, *dict(KEEP, src=C.byref(a), dst=C.byref(b)).values())
     c = cache(kd=260)
     refused("gllm_hip_kv_keep_dev", g.EUNSUP, *dict(KEEP, src=C.byref(a), dst=C.byref(c)).values())
+    big, to = cache(kd=1 << 20, vd=1 << 20, rows=1 << 20), cache(kd=1 << 20, vd=1 << 20, rows=1 << 20)
+    refused("gllm_hip_kv_keep_dev", g.EUNSUP, *dict(KEEP, src=C.byref(big), dst=C.byref(to), kvh=1 << 14, len=1 << 20, budget=1 << 20,
+                                                    stride=1 << 20, out_stride=1 << 20).values())
+    far = cache(rows=(1 << 30) + 1)
+    refused("gllm_hip_kv_keep_dev", g.EUNSUP, *dict(KEEP, src=C.byref(far), dst=C.byref(a)).values())
+    refused("gllm_hip_kv_evict_store_dev", g.EUNSUP, *dict(EVICT, kv=C.byref(far)).values())
 
 
 EVICT = dict(kv=None, l=0, kvh=2, hd=64, k=P, v=P, start=0, len=50, sinks=1, recent=2, mass=P, pos=P, stride=100, now=P, rows=None,

@@ -302,6 +302,69 @@ def test_mass(hip, n, heads, n_kv, hd, start, end):
     assert abs((got_mass - before)[:, live].sum() - total) <= 1e-4 * total + 1e-5 * rows
 
 
+@pytest.mark.parametrize("n,heads,n_kv,hd,end", [(3, 2, 1, 64, 50), (4, 8, 2, 128, 31), (20, 8, 2, 128, 65), (40, 4, 1, 96, 130), (5, 2, 2, 40, 4)])
+def test_mass_rows_that_only_later_tokens_see(hip, n, heads, n_kv, hd, end):
+    """Infinities and NaN in the last tokens' own rows stay out of the tokens before."""
+    kv, k, v = make_cache(hip, end + 3, n_kv * hd, 530, live=[(0, end - 1)])  # the last two tokens' rows are not finite
+    import torch
+    q, out = normal(531, (n, heads * hd)), torch.empty((n, heads * hd), device="cuda")
+    mass = torch.zeros((n_kv, end + 1), device="cuda")
+    print(f"mass, later rows not finite: n {n} heads {heads}/{n_kv}x{hd} end {end}", flush=True)
+    kv.attend_mass_dev(0, cuda(q), heads, n_kv, hd, 0, end, hd ** -0.5, mass, out)
+    got = host(out)
+    for i in range(n - 2):
+        want, _, u, vm = attend64(q[i], k, v, np.arange(end - (n - 1) + i + 1), hd, n_kv, hd ** -0.5)
+        assert np.abs(got[i] - want).max() <= u * vm, i
+
+
+def test_capture_without_a_workspace_needs_an_earlier_call(hip):
+    """The library's scratch does not grow under capture: the call is refused and captures nothing."""
+    import torch
+    kv, _, _ = make_cache(hip, 5000, 128, 540)
+    q, out = torch.zeros((2, 512), device="cuda"), torch.full((2, 512), 7.0, device="cuda")
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    x = torch.zeros(4, device="cuda")
+    with torch.cuda.graph(graph, stream=side):
+        x.add_(1.0)
+        with pytest.raises(hip.GllmError) as e:
+            kv.attend_shared_dev(0, q, 8, 2, 64, 0, 5000, None, None, 0, 0.1, out)
+        assert e.value.code == hip.EUNSUP
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (out == 7.0).all() and (x == 1.0).all()
+    hip.stream_release(side.cuda_stream)
+
+
+def test_two_host_threads_at_once(hip):
+    """Calls of two threads on two streams over one cache, each with the library's scratch of its own."""
+    import threading
+    import torch
+    kv, k, v = make_cache(hip, 900, 256, 550)
+    qs = [normal(551 + i, (9, 512)) for i in range(2)]
+    wants = [[attend64(q[t], k, v, np.arange(900), 64, 4, 0.125) for t in range(9)] for q in qs]
+    bad = []
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            dq, out = cuda(qs[i]), torch.empty((9, 512), device="cuda")
+            for _ in range(20):
+                kv.attend_shared_dev(0, dq, 8, 4, 64, 0, 900, None, None, 0, 0.125, out)
+            s.synchronize()
+            got = out.cpu().numpy()
+        for t, (want, _, u, vm) in enumerate(wants[i]):
+            if not np.abs(got[t] - want).max() <= u * vm:
+                bad.append((i, t))
+        hip.stream_release(s.cuda_stream)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
 def test_mass_adds_up_over_calls_and_replays(hip):
     """Two eager calls and three replays of a captured one add five times the weights."""
     import torch
