@@ -26,15 +26,22 @@ struct SeqPlan {
 
 inline int ceil_div(int a, int b) { return (int)(((long long)a + b - 1) / b); }
 
-// n tokens, heads / kv heads, `len` shared positions, own ranges planned for
+// n tokens, heads / kv heads of hd, `len` shared positions, own ranges planned for
 // `most` positions (0: none).
-inline SeqPlan seq_plan(int n, int n_heads, int n_kv, int len, int most) {
+inline SeqPlan seq_plan(int n, int n_heads, int n_kv, int hd, int len, int most) {
     SeqPlan p{};
     p.r = n_heads / n_kv;
     p.rows = (size_t)n * n_heads;
     const long long per_kv = (long long)n * p.r;
-    p.nq = per_kv <= 64 ? 1 : 2;
+    // Up to 16 rows: the waves split positions.  More: they share the positions,
+    // 16 rows each, or 32 where that leaves no more padding and there is work
+    // enough that reading the tiles half as often counts.  With 16 and 32 rows, 8
+    // kv heads of 128, rows x positions: 256 x 32768 81 and 73 us, 1024 x 4000 59
+    // and 54, 256 x 16000 50 and 51, 128 x 32768 48 and 49, 256 x 8000 33 and 36,
+    // 128 x 8000 22 and 28.
     p.rw = per_kv <= 16 ? 1 : kSeqWaves;
+    const bool fits = (per_kv + 63) / 64 * 64 == (per_kv + 127) / 128 * 128;
+    p.nq = fits && per_kv * (double)len * n_kv * hd > 4.0e9 ? 2 : 1;
     p.row_blocks = (int)((per_kv + 16 * p.nq * p.rw - 1) / (16 * p.nq * p.rw));
     if (len > 0) {
         const long long per_chunk = (long long)n_kv * p.row_blocks;

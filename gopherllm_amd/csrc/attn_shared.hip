@@ -799,7 +799,7 @@ size_t gllm_hip_attend_shared_bytes(int n, int n_heads, int n_kv_heads, int hd, 
     if (n < 1 || n_kv_heads < 1 || n_heads < 1 || n_heads % n_kv_heads || hd < 1 || hd > 128 || len < 0 || most < 0 ||
         (long long)n * n_heads > kSeqMaxRows)
         return 0;
-    return 4 * seq_floats(seq_plan(n, n_heads, n_kv_heads, len, most), hd);
+    return 4 * seq_floats(seq_plan(n, n_heads, n_kv_heads, hd, len, most), hd);
 }
 
 int gllm_hip_attend_shared_dev(gllm_hip_kv* kv, int l, const float* d_q, int n, int n_heads, int n_kv_heads, int hd,
@@ -812,7 +812,7 @@ int gllm_hip_attend_shared_dev(gllm_hip_kv* kv, int l, const float* d_q, int n, 
     if (most < 0 || (most > 0) != (d_starts != nullptr) || (most > 0) != (d_lens != nullptr))
         return fail(GLLM_EINVAL, "%s: own rows need starts, lens and most > 0 together", what);
     hipStream_t s = (hipStream_t)stream;
-    const SeqPlan p = seq_plan(n, n_heads, n_kv_heads, len, most);
+    const SeqPlan p = seq_plan(n, n_heads, n_kv_heads, hd, len, most);
     float* w;
     GLLM_TRY(seq_work(what, kv, seq_floats(p, hd), d_work, work_bytes, s, &w));
     SeqArgs a = seq_args(kv, l, d_q, n, n_heads, n_kv_heads, hd, scale, p, w);
@@ -830,7 +830,7 @@ size_t gllm_hip_attend_mass_bytes(int n, int n_heads, int n_kv_heads, int hd, in
     if (n < 1 || n_kv_heads < 1 || n_heads < 1 || n_heads % n_kv_heads || hd < 1 || hd > 128 || len < 1 ||
         n > len || (long long)n * n_heads > kSeqMaxRows)
         return 0;
-    return 4 * mass_floats(seq_plan(n, n_heads, n_kv_heads, len - (n - 1), n - 1), hd, n_kv_heads, len);
+    return 4 * mass_floats(seq_plan(n, n_heads, n_kv_heads, hd, len - (n - 1), n - 1), hd, n_kv_heads, len);
 }
 
 int gllm_hip_attend_mass_dev(gllm_hip_kv* kv, int l, const float* d_q, int n, int n_heads, int n_kv_heads, int hd,
@@ -844,7 +844,7 @@ int gllm_hip_attend_mass_dev(gllm_hip_kv* kv, int l, const float* d_q, int n, in
     hipStream_t s = (hipStream_t)stream;
     const int len = end - start + 1;
     // what every token attends is the shared range; token i has i rows more
-    const SeqPlan p = seq_plan(n, n_heads, n_kv_heads, len - (n - 1), n - 1);
+    const SeqPlan p = seq_plan(n, n_heads, n_kv_heads, hd, len - (n - 1), n - 1);
     float* w;
     GLLM_TRY(seq_work(what, kv, mass_floats(p, hd, n_kv_heads, len), d_work, work_bytes, s, &w));
     const MassSpace m = mass_space(p, hd, n_kv_heads, len);

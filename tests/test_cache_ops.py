@@ -29,7 +29,7 @@ int main() {
     for (int n : ns) for (int r : rs) for (int g : gs) for (int len : lens) for (int most : lens) {
         const int h = r * g;
         if ((long long)n * h > (1 << 24)) continue;
-        const SeqPlan p = seq_plan(n, h, g, len, most);
+        const SeqPlan p = seq_plan(n, h, g, r % 2 ? 128 : 40, len, most);
         plans++;
         need(p.r == r && p.rows == (size_t)n * h, "rows", n, h, g, len, most);
         need((long long)p.row_blocks * 16 * p.nq * p.rw >= (long long)n * r, "row blocks", n, h, g, len, most);

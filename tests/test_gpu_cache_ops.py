@@ -194,6 +194,53 @@ def test_shared_workspace_is_the_callers(hip):
     assert (out == 7.0).all()
 
 
+def bound64(q, k, hd, scale):
+    """The tolerance's u for float64 device tensors q (rows, hd) and k (positions, hd)."""
+    s_max = float((q.abs() @ k.abs().T.contiguous()).max()) * abs(scale)
+    return 2 * (s_max * (2.0 ** -22 + (math.sqrt(hd) + 1) * 2.0 ** -23) + 2.0 ** -20)
+
+
+# enough work for 32 query rows a wave: over 4e9 rows x positions x head size
+@pytest.mark.parametrize("n,r,hd,length", [(1024, 8, 128, 4001), (2048, 8, 80, 3201), (2048, 8, 40, 6503), (2048, 8, 24, 10901), (63, 65, 128, 7815)])
+def test_shared_many_rows_over_long_prefixes(hip, n, r, hd, length):
+    import torch
+    most = 3
+    kv, k, v = make_cache(hip, length + most * n + 1, hd, 375)
+    q = normal(376, (n, r * hd))
+    starts = cuda((length + most * np.arange(n)).astype(np.int32))
+    lens = cuda((np.arange(n) % (most + 1)).astype(np.int32))
+    out = torch.empty((n, r * hd), device="cuda")
+    print(f"shared, many rows: {n} x {r} x {hd} over {length}", flush=True)
+    kv.attend_shared_dev(0, cuda(q), r, 1, hd, 0, length, starts, lens, most, hd ** -0.5, out)
+    q64, k64, v64 = cuda(q).double().view(n, r, hd), cuda(k), cuda(v)
+    rows = starts.long()[:, None] + torch.arange(most, device="cuda")
+    s = torch.cat([(q64.view(-1, hd) @ k64[:length].T.contiguous()).view(n, r, length), (q64[:, :, None] * k64[rows][:, None]).sum(-1)], -1) * hd ** -0.5
+    s[..., length:].masked_fill_((torch.arange(most, device="cuda") >= lens[:, None])[:, None], -math.inf)
+    w = torch.softmax(s, -1)
+    want = (w[..., :length].reshape(-1, length) @ v64[:length]).view(n, r, hd) + (w[..., length:, None] * v64[rows][:, None]).sum(2)
+    u = bound64(q64.view(-1, hd), k64, hd, hd ** -0.5)
+    assert float((out.double().view(n, r, hd) - want).abs().max()) <= u * float(v64.abs().max())
+
+
+def test_mass_many_rows_over_a_long_prefix(hip):
+    import torch
+    n, r, hd, length = 1024, 8, 128, 5200
+    kv, k, v = make_cache(hip, length, hd, 377)
+    q = normal(378, (n, r * hd))
+    out, mass = torch.empty((n, r * hd), device="cuda"), torch.zeros((1, length), device="cuda")
+    print("mass, many rows", flush=True)
+    kv.attend_mass_dev(0, cuda(q), r, 1, hd, 0, length - 1, hd ** -0.5, mass, out)
+    q64, k64, v64 = cuda(q).double().view(-1, hd), cuda(k), cuda(v)
+    s = (q64 @ k64.T.contiguous()).view(n, r, length) * hd ** -0.5
+    s.masked_fill_((torch.arange(length, device="cuda") > length - n + torch.arange(n, device="cuda")[:, None])[:, None], -math.inf)
+    w = torch.softmax(s, -1)
+    want, per = w.view(-1, length) @ v64, w.sum((0, 1))
+    u = bound64(q64, k64, hd, hd ** -0.5)
+    assert float((out.double().view(-1, hd) - want).abs().max()) <= u * float(v64.abs().max())
+    # n * r additions, tile by tile: at most as many roundings as the sum has terms
+    assert bool(((mass[0].double() - per).abs() <= (u + n * r * 2.0 ** -24) * per).all())
+
+
 def test_shared_agrees_with_the_single_sequence(hip):
     """n equal requests over a prefix are n times attend_dev over the same rows."""
     import torch
