@@ -647,21 +647,28 @@ __global__ __launch_bounds__(256, 2) void seq_mass_kernel(MassArgs a) {
     for (int t = 0; t < PT; t++) sum[t] = f4{0, 0, 0, 0};
     const u4* parts = a.q_parts + (size_t)g * a.tiles * 2 * KK * 64 + lane;
     const int rows = a.n * a.r, tiles = (rows + 15) / 16;
+    // a tile's operands, and its rows' scale, base and 1 / sum, are read one tile ahead
     u4 next[2 * KK];
+    float2 next_b;
+    float next_c;
+    int next_i;
+    const auto load = [&](int tile) {
 #pragma unroll
-    for (int i = 0; i < 2 * KK; i++) next[i] = parts[i * 64];
+        for (int j = 0; j < 2 * KK; j++) next[j] = parts[(tile * 2 * KK + j) * 64];
+        const int rr = min(16 * tile + col, rows - 1);
+        next_i = rr / a.r;
+        next_b = a.ml[(size_t)next_i * a.n_heads + g * a.r + (rr - next_i * a.r)];
+        next_c = a.q_scale[((size_t)g * a.tiles + tile) * 16 + col];
+    };
+    load(0);
     for (int tile = 0; tile < tiles; tile++) {
         h8 q[2 * KK];
 #pragma unroll
         for (int i = 0; i < 2 * KK; i++) q[i] = __builtin_bit_cast(h8, next[i]);
-        const int rr = 16 * tile + col, i = min(rr, rows - 1) / a.r;
-        const float2 b = a.ml[(size_t)i * a.n_heads + g * a.r + (min(rr, rows - 1) - i * a.r)];
-        const float c = a.q_scale[((size_t)g * a.tiles + tile) * 16 + col], inv = rr < rows ? b.y : 0.0f;
-        const int lim = a.len - (a.n - 1 - i);  // positions from it on are masked
-        if (tile + 1 < tiles) {
-#pragma unroll
-            for (int j = 0; j < 2 * KK; j++) next[j] = parts[((tile + 1) * 2 * KK + j) * 64];
-        }
+        const float2 b = next_b;
+        const float c = next_c, inv = 16 * tile + col < rows ? b.y : 0.0f;
+        const int lim = a.len - (a.n - 1 - next_i);  // positions from it on are masked
+        if (tile + 1 < tiles) load(tile + 1);
         f4 s[PT];
 #pragma unroll
         for (int t = 0; t < PT; t++) s[t] = f4{0, 0, 0, 0};
@@ -686,8 +693,10 @@ __global__ __launch_bounds__(256, 2) void seq_mass_kernel(MassArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             float x = sum[t][j];
-#pragma unroll
-            for (int off = 8; off >= 1; off >>= 1) x += __shfl_xor(x, off);
+            x += dpp_f<kQuadXor1>(x);
+            x += dpp_f<kQuadXor2>(x);
+            x += dpp_f<kRowHalfMirror>(x);
+            x += dpp_f<kRowMirror>(x);
             const int p = p0 + 16 * t + 4 * grp + j;
             if (col == 0 && p < a.len) a.mass[(size_t)g * a.mass_stride + p] += x;
         }
