@@ -687,7 +687,8 @@ __global__ __launch_bounds__(256, 2) void seq_mass_kernel(MassArgs a) {
                 sum[t][j] += p0 + 16 * t + 4 * grp + j < lim ? w : 0.0f;
             }
     }
-    // over the 16 rows of the tiles; position 16 t + 4 grp + j
+    // over the 16 rows of the tiles; lane col keeps position 16 (col / 4) + 4 grp + col % 4
+    float mine = 0.0f;
 #pragma unroll
     for (int t = 0; t < PT; t++)
 #pragma unroll
@@ -697,9 +698,10 @@ __global__ __launch_bounds__(256, 2) void seq_mass_kernel(MassArgs a) {
             x += dpp_f<kQuadXor2>(x);
             x += dpp_f<kRowHalfMirror>(x);
             x += dpp_f<kRowMirror>(x);
-            const int p = p0 + 16 * t + 4 * grp + j;
-            if (col == 0 && p < a.len) a.mass[(size_t)g * a.mass_stride + p] += x;
+            mine = col == 4 * t + j ? x : mine;
         }
+    const int p = p0 + 16 * (col >> 2) + 4 * grp + (col & 3);
+    if (p < a.len) a.mass[(size_t)g * a.mass_stride + p] += mine;
 }
 
 template <int NQ, int RW>
