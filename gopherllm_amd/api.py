@@ -510,7 +510,9 @@ class KVCacheF16:
         return out
 
     def tensors(self, layer):
-        """(K, V) of a layer as float16 tensors of max_len rows over the cache's own memory."""
+        """(K, V) of a layer as float16 tensors of max_len rows over the cache's own
+        memory: they hold this object, and end with release() (or, for a decoder's
+        cache, with the decoder)."""
         import torch
         if not 0 <= layer < self.layers:
             raise ValueError(f"tensors: layer {layer} of {self.layers}")

@@ -16,11 +16,11 @@
 // the weights, so that the second part stays normal where it counts.
 //
 // A workgroup's four waves split the positions of a chunk, or its query rows
-// where there are many.  Per 32 positions a wave forms the transposed scores S^T = K Q^T and the transposed output
-// O^T += V^T W^T: the accumulator layout of S^T (query = lane & 15, position
-// = 4 * (lane / 16) + register) is, for two tiles of 16 positions, the
-// operand layout of W^T, so the weights never leave the lane.  V^T is read
-// from an LDS tile with the transposing loads.
+// where there are many.  Per 32 positions a wave forms the transposed scores
+// S^T = K Q^T and the transposed output O^T += V^T W^T: the accumulator layout
+// of S^T (query = lane & 15, position = 4 * (lane / 16) + register) is, for two
+// tiles of 16 positions, the operand layout of W^T, so the weights never leave
+// the lane.  V^T is read from an LDS tile with the transposing loads.
 #include <algorithm>
 
 #include "attn_plan.h"
@@ -310,8 +310,10 @@ __device__ __forceinline__ size_t seq_part(const SeqArgs& a, bool own, int g, in
 
 // Up to 16 query rows: the four waves take different positions, each with K
 // straight from memory into operand order and V through its own LDS tile, and
-// join their sums in LDS.  HD: head size rounded up to 32 (hd <= HD,
-// hd % 8 == 0); OWN: each token's own rows, not the shared ones.
+// join their sums in LDS.  Bound by memory: one request over 32768 rows of 8
+// kv heads of 128 (134 MB) takes 26 us with the joining launch, 5.1 TB/s.
+// HD: head size rounded up to 32 (hd <= HD, hd % 8 == 0); OWN: each token's own
+// rows, not the shared ones.
 template <int HD, bool OWN>
 __device__ __forceinline__ void seq_few(const SeqArgs& a, int b, char* lds, float (*sm)[16], float (*sl)[16]) {
     constexpr int KK = HD / 32, DT = HD / 16, CH = HD / 8, LD = kStep * CH / 64;
@@ -427,8 +429,11 @@ __device__ __forceinline__ void seq_few(const SeqArgs& a, int b, char* lds, floa
 
 // Many query rows: the four waves take 16 NQ rows each over the same positions
 // and share the K and V tiles, which direct copies bring into a ring of stages
-// three steps ahead (registers for one step ahead left the kernel waiting on
-// memory: 64 requests over 32768 rows took 85 us).
+// three steps ahead (with registers, one step ahead, 64 requests over 32768 rows
+// took 85 us).  Bound by the matrix cores: 256 rows of each of 8 kv heads over
+// 32768 positions take 73 us, 54 of them in this loop: 69 GFLOP at 1270
+// TFLOP/s, the rate of a large library product here; the rest is the launch,
+// the queries, the first tiles (10 us) and the partial results (8).
 template <int HD, int NQ>
 __device__ __forceinline__ void seq_many(const SeqArgs& a, int b, char* lds) {
     constexpr int KK = HD / 32, DT = HD / 16, CH = HD / 8, TILE = SeqLds<HD, 4>::TILE;
@@ -542,7 +547,7 @@ struct MergeArgs {
     const float *pm, *pl, *po;
     float* out;
     float2* ml;           // base and 1 / sum of each row, or null
-    int rows, slots, hd;
+    int slots, hd;
     const float* scores;  // one token: [row][sstride], or null
     float* mass;          // [kv head][mass_stride], from the first attended row on
     int sstride, n, n_heads, n_kv, r, len, mass_stride, mass_wgs;
@@ -620,9 +625,9 @@ struct MassArgs {
 
 // The weights of several tokens, from their scores made again: a wave holds 64
 // positions' keys in registers and takes the rows' operands, 16 rows at a time,
-// as the attention left them.  Reading K twice (33 MB for 16001 rows of 8 heads
-// of 128) costs less than writing and reading the scores of 32 tokens (65 MB each
-// way: 44 + 40 us for both kernels).
+// as the attention left them.  For 32 tokens over 16001 rows of 8 heads of 128
+// this takes 17.5 us; writing their scores (65 MB) took the attention 16 us
+// more, and reading them 35.
 template <int HD>
 __global__ __launch_bounds__(256, 2) void seq_mass_kernel(MassArgs a) {
     constexpr int KK = HD / 32, PT = 4;
@@ -777,7 +782,6 @@ static MergeArgs merge_args(const SeqArgs& a, const SeqPlan& p, float* d_out) {
     m.pl = a.pl;
     m.po = a.po;
     m.out = d_out;
-    m.rows = (int)p.rows;
     m.slots = p.slots;
     m.hd = a.hd;
     m.n = a.n;
