@@ -454,7 +454,7 @@ ROPES = [
     (2, 3, 1, 8, dict(rot_dim=2)), (300, 4, 2, 128, dict(scaling="llama3", factor=8.0, orig_ctx=8192)),
     (9, 2, 1, 50, dict(rot_dim=26, scaling="linear", factor=3.0, attn_factor=0.5)),
     (4, 2, 2, 66, dict(rot_dim=66, layout="half", freq_factors=np.linspace(1, 4, 33, dtype=np.float32))),
-    (5, 1, 1, 1024, dict(theta=10000.0)),
+    (5, 1, 1, 1024, dict(theta=10000.0)), (2, 300, 2, 1024, dict(layout="half")), (3, 6, 2, 64, dict(rot_dim=20, layout="half")),
 ]
 
 
@@ -538,6 +538,19 @@ def test_rope_turns_as_the_decoder_does(hip):
     hip.Rope(64).apply_dev(t, cuda(np.array([3], np.int32)))
     # the decoder's frequencies and angle are float32: 2 roundings of an angle up to 3
     assert np.abs(host(t)[0] - want).max() <= np.abs(x).max() * (3 * 2 * 2.0 ** -24 + 6 * 2.0 ** -24)
+
+
+def test_rope_in_quads_and_strided(hip):
+    """Aligned rows of a fused projection (quads) against the same values one row off (pairs)."""
+    import torch
+    rope = hip.Rope(64, rot_dim=32, layout="half")
+    x = cuda(normal(640, (9, 3 * 64 + 8)))
+    pos = cuda(rope_positions(9, 641))
+    quads = rope.apply_dev(x[:, :192], pos, torch.empty((9, 192), device="cuda"))
+    odd = torch.empty((9, 3 * 64 + 7), device="cuda")
+    odd[:, 1:193].copy_(x[:, :192])
+    pairs = rope.apply_dev(odd[:, 1:193], pos, torch.empty((9, 193), device="cuda")[:, 1:])
+    assert np.array_equal(host(quads), host(pairs))
 
 
 def test_rope_no_tokens_and_refusals(hip):
