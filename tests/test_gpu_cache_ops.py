@@ -690,6 +690,54 @@ def test_evict_gives_up_nan_first(hip):
     assert host(victims)[0] == 66
 
 
+def test_far_rows_of_a_long_cache(hip):
+    """Store, weights, keeping and evicting at rows past 4 GiB of K and of V (and 2^31 values)."""
+    import torch
+    rows, n_kv, hd = 1_100_000, 16, 128
+    dim = n_kv * hd
+    kv, small = hip.KVCacheF16(1, dim, dim, rows), hip.KVCacheF16(1, dim, dim, 10)
+    n = 40
+    a = rows - n
+    rope = hip.Rope(hd)
+    inv, amp = hip.Rope.frequencies(hd)
+    k, v = normal(850, (n, dim)), normal(851, (n, dim))
+    pos = np.arange(n, dtype=np.int32)
+    print("far rows: store", flush=True)
+    kv.store_rope_dev(0, rope, None, cuda(k), cuda(v), cuda(pos), cuda((a + pos).astype(np.int32)))
+    tk, tv = kv.tensors(0)
+    k16, v16 = host(tk[a:]), host(tv[a:])
+    assert np.abs(k16 - rotate64(k, pos, inv, amp, hd, False)).max() <= np.abs(k).max() * 2.0 ** -10
+    assert np.array_equal(v16, v.astype(np.float16)) and not host(tk[:n]).any() and not host(tv[:n]).any()
+    k64, v64 = k16.astype(np.float64), v16.astype(np.float64)
+    for tokens in (1, 3):  # scores kept, and made again
+        q, out = normal(852, (tokens, 2 * dim)), torch.empty((tokens, 2 * dim), device="cuda")
+        mass = torch.zeros((n_kv, rows), device="cuda")
+        print(f"far rows: weights of {tokens}", flush=True)
+        kv.attend_mass_dev(0, cuda(q), 2 * n_kv, n_kv, hd, a, rows - 1, hd ** -0.5, mass, out)
+        got, want = host(mass), np.zeros((n_kv, n))
+        for i in range(tokens):
+            at = np.arange(n - tokens + i + 1)
+            o, w, u, vm = attend64(q[i], k64, v64, at, hd, n_kv, hd ** -0.5)
+            want[:, at] += w.reshape(n_kv, 2, -1).sum(1)
+            assert np.abs(host(out)[i] - o).max() <= u * vm
+        assert np.abs(got[:, a:] - want).max() <= (u + 2.0 ** -20) * want.max() and not got[:, :a].any()
+    m2, p2 = torch.zeros((1, n_kv, 10), device="cuda"), torch.zeros((1, n_kv, 10), dtype=torch.int32, device="cuda")
+    print("far rows: keep", flush=True)
+    kv.keep_dev(small, n_kv, hd, n, 10, mass[None], None, m2, p2, now=rows, start=a)
+    sk = host(small.tensors(0)[0])
+    for g in range(n_kv):
+        best = np.sort(order_of(got[g, a:], np.arange(a, rows), 0, rows)[:10])
+        assert np.array_equal(host(p2)[0, g], a + best) and np.array_equal(sk[:, g * hd:g * hd + hd], k16[best, g * hd:g * hd + hd])
+    positions = torch.arange(rows, dtype=torch.int32, device="cuda").repeat(n_kv, 1)
+    gone, now = torch.zeros(n_kv, dtype=torch.int32, device="cuda"), torch.full((1,), rows, dtype=torch.int32, device="cuda")
+    print("far rows: evict", flush=True)
+    kv.evict_store_dev(0, n_kv, hd, cuda(k[0]), cuda(v[0]), a, n, mass, positions, now, rows_out=gone)
+    for g in range(n_kv):
+        t = int(np.argmin(got[g, a:]))
+        assert host(gone)[g] == a + t
+        assert np.array_equal(host(tv[a + t])[g * hd:g * hd + hd], v[0, g * hd:g * hd + hd].astype(np.float16))
+
+
 # --- a run of them together ------------------------------------------------------------
 
 
