@@ -798,3 +798,46 @@ def test_a_bounded_cache_from_prompt_to_decode(hip):
             o, w, _, _ = attend64(q64[at, hs], k16[:, c], v16[:, c], rows[g], hd, 1, scale)
             assert np.abs(host(o1)[0, hs] - o).max() <= 2e-3
             assert np.allclose(host(m2)[0, g], before[g] + w.sum(0), rtol=1e-2, atol=1e-6)
+
+
+def test_a_captured_decode_step(hip):
+    """Rotation, eviction and weighted attention of a step in one graph, replayed as tokens and positions
+    change under it with other work in between: the same bits as the eager calls on a second cache."""
+    import torch
+    heads, n_kv, hd, budget = 8, 2, 64, 70
+    dim = n_kv * hd
+    rope = hip.Rope(hd, layout="half")
+    sides = []
+    for _ in range(2):
+        kv, _, _ = make_cache(hip, budget, dim, 950)
+        st = {"kv": kv, "mass": cuda(np.abs(normal(951, (n_kv, budget)))), "pos": cuda(np.tile(np.arange(budget, dtype=np.int32), (n_kv, 1))),
+              "now": torch.zeros(1, dtype=torch.int32, device="cuda"), "q": torch.zeros((1, heads * hd), device="cuda"),
+              "k": torch.zeros((1, dim), device="cuda"), "v": torch.zeros((1, dim), device="cuda"),
+              "qr": torch.zeros((1, heads * hd), device="cuda"), "kr": torch.zeros((1, dim), device="cuda"),
+              "out": torch.zeros((1, heads * hd), device="cuda"),
+              "work": torch.empty(hip.attend_mass_bytes(1, heads, n_kv, hd, budget), dtype=torch.uint8, device="cuda")}
+        sides.append(st)
+
+    def step(st):
+        rope.apply_dev(st["q"], st["now"], st["qr"])
+        rope.apply_dev(st["k"], st["now"], st["kr"])
+        st["kv"].evict_store_dev(0, n_kv, hd, st["kr"], st["v"], 0, budget, st["mass"], st["pos"], st["now"], sinks=4, recent=16)
+        st["kv"].attend_mass_dev(0, st["qr"], heads, n_kv, hd, 0, budget - 1, hd ** -0.5, st["mass"], st["out"], work=st["work"])
+
+    eager, captured = sides
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=stream):
+        step(captured)
+    for i in range(6):
+        x = [cuda(normal(960 + 3 * i + j, (1, w))) for j, w in enumerate((heads * hd, dim, dim))]
+        for st in sides:
+            for name, t in zip(("q", "k", "v"), x):
+                st[name].copy_(t)
+            st["now"].fill_(budget + i)
+        step(eager)
+        torch.ones(5000, device="cuda").sum()
+        graph.replay()
+        for name in ("out", "mass", "pos"):
+            assert np.array_equal(host(eager[name]), host(captured[name])), (i, name)
+        for a, b in zip(eager["kv"].tensors(0), captured["kv"].tensors(0)):
+            assert np.array_equal(host(a), host(b)), i
