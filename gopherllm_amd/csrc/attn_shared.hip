@@ -671,8 +671,10 @@ __global__ __launch_bounds__(256, 2) void seq_mass_kernel(MassArgs a) {
 #pragma unroll
         for (int i = 0; i < 2 * KK; i++) q[i] = __builtin_bit_cast(h8, next[i]);
         const float2 b = next_b;
-        const float c = next_c, inv = 16 * tile + col < rows ? b.y : 0.0f;
-        const int lim = a.len - (a.n - 1 - next_i);  // positions from it on are masked
+        const float c = next_c, inv = b.y;
+        // positions from lim on are masked, all of them for a row that only fills the
+        // tile: its dots are 0 and its base another row's, so its weight can be Inf
+        const int lim = 16 * tile + col < rows ? a.len - (a.n - 1 - next_i) : 0;
         if (tile + 1 < tiles) load(tile + 1);
         f4 s[PT];
 #pragma unroll
