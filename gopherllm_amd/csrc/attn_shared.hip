@@ -9,11 +9,13 @@
 //   out   = sum w_p v_p / sum w_p     over the shared rows, then the own rows
 //
 // K and V are f16 and q and w are float32.  Each of q and w is the sum of two
-// f16 values (its rounding and the rounding of the rest, 22 bits), so two
+// f16 values (its rounding and the rounding of the rest, both to nearest: off by
+// at most 2^-23 of its power of two), so two
 // f16 matrix products, whose products are exact in the float32 accumulator,
 // stand for one float32 product at an eighth of its matrix-core time.  q is
 // first scaled by a power of two to a maximum in [2^14, 2^15), and base lifts
-// the weights, so that the second part stays normal where it counts.
+// the weights, so that the second part stays normal where it counts: below,
+// f16's step of 2^-24 leaves a weight off by up to 2^-33 of the row's largest.
 //
 // A workgroup's four waves split the positions of a chunk, or its query rows
 // where there are many.  Per 32 positions a wave forms the transposed scores
@@ -33,6 +35,8 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 struct SeqArgs {
@@ -62,7 +66,10 @@ struct SeqArgs {
 
 // A new base puts the largest weight so far at 2^8; it stays until a weight
 // would pass 2^15, so that most steps leave the sums as they are (f16 ends at
-// 2^16; at the other end a weight's second part ends 2^-32 below the largest).
+// 2^16).  At the other end a weight's second part is rounded to f16's steps of
+// 2^-24, 2^-33 of the largest weight, to nearest: cut towards zero, which takes as
+// long, the losses of many small weights add up (rows 2^18 below the heaviest
+// ones came out 2.7e-5 low, now 1e-6 either way).
 constexpr float kSeqLift = 8.0f, kSeqRoom = 15.0f;
 constexpr float kNoBase = -3.0e38f;  // of a query without positions so far: every factor of its zero sums is finite
 constexpr int kBufferWord3 = 0x00020000;  // raw buffer of 32-bit data; reads past its end give 0
@@ -247,16 +254,17 @@ __device__ __forceinline__ void seq_step(const SeqArgs& a, int g, int row0, int 
         for (int t = 0; t < 2; t++)
 #pragma unroll
             for (int j = 0; j < 4; j += 2) {
-                // the two parts of a weight, both cut short: 21 bits
+                // the two parts of a weight, to nearest (what cannot be held must not
+                // all be on one side)
                 const float w0 = __builtin_amdgcn_exp2f(fmaf(s[nq][t][j], cc[nq], -q.base[nq]));
                 const float w1 = __builtin_amdgcn_exp2f(fmaf(s[nq][t][j + 1], cc[nq], -q.base[nq]));
                 q.l[nq] += w0 + w1;
-                const auto hi = __builtin_amdgcn_cvt_pkrtz(w0, w1);
-                const auto lo = __builtin_amdgcn_cvt_pkrtz(fmaf((float)hi[0], minus1, w0), fmaf((float)hi[1], minus1, w1));
-                wh[nq][4 * t + j] = (_Float16)hi[0];
-                wh[nq][4 * t + j + 1] = (_Float16)hi[1];
-                wl[nq][4 * t + j] = (_Float16)lo[0];
-                wl[nq][4 * t + j + 1] = (_Float16)lo[1];
+                const h2 hi = __builtin_convertvector((f2{w0, w1}), h2);
+                const h2 lo = __builtin_convertvector((f2{fmaf((float)hi[0], minus1, w0), fmaf((float)hi[1], minus1, w1)}), h2);
+                wh[nq][4 * t + j] = hi[0];
+                wh[nq][4 * t + j + 1] = hi[1];
+                wl[nq][4 * t + j] = lo[0];
+                wl[nq][4 * t + j + 1] = lo[1];
             }
     // V operand k = 8 grp + 4 t + j is position 16 t + 4 grp + j
     const int vr = 4 * grp + (col >> 2);

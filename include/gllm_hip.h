@@ -333,10 +333,11 @@ int gllm_hip_kv_store_rope_dev(gllm_hip_kv* kv, int l, const gllm_hip_rope* r, c
  * with null arrays: no own rows, as for cross attention to an encoder's
  * states.  Ranges may overlap: several tokens of one request are several
  * requests whose own ranges start together (a row in both ranges counts
- * twice).  A request without any row gets zeros.  Sums are float32, products
- * of 22-bit q and weights.  Rows outside a request's ranges may hold anything;
- * where an attended row holds an infinity or NaN the outputs of its kv head are
- * not defined. */
+ * twice).  A request without any row gets zeros.  Sums are float32; q and the
+ * weights enter the products rounded to 2^-23 of their power of two, a weight
+ * also to 2^-33 of the request's largest, all to nearest.  Rows outside a
+ * request's ranges may hold anything; where an attended row holds an infinity
+ * or NaN the outputs of its kv head are not defined. */
 size_t gllm_hip_attend_shared_bytes(int n, int n_heads, int n_kv_heads, int hd, int len, int most);
 int gllm_hip_attend_shared_dev(gllm_hip_kv* kv, int l, const float* d_q, int n, int n_heads,
                                int n_kv_heads, int hd, int start, int len,
