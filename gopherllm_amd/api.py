@@ -77,14 +77,14 @@ def _here():
     tensors' device.  A decode step makes a few such calls per layer, each a few
     microseconds on the GPU, so they look torch up once and ask it for plain
     numbers (a torch Stream object alone is 3 us)."""
-    global _torch, _raw_stream
+    global _kinds, _torch, _raw_stream
     if not _kinds:
         import torch
-        for kind, names in _DTYPES.items():
-            _kinds[kind] = frozenset(getattr(torch, n) for n in names if hasattr(torch, n))
+        kinds = {kind: frozenset(getattr(torch, n) for n in names if hasattr(torch, n)) for kind, names in _DTYPES.items()}
         _torch = torch
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
                               lambda at: torch.cuda.current_stream(at).cuda_stream)
+        _kinds = kinds  # last and whole: another thread that sees it sees the others
     at = _torch.cuda.current_device()
     return at, _raw_stream(at)
 
