@@ -79,6 +79,7 @@ SIGNATURES = {
     "gllm_hip_kv_release": (None, [vp]),
     "gllm_hip_kv_k_dev": (vp, [vp, i32]),
     "gllm_hip_kv_v_dev": (vp, [vp, i32]),
+    "gllm_hip_kv_device": (i32, [vp]),
     "gllm_hip_kv_read": (i32, [vp, i32, i32, i32, vp, vp]),
     "gllm_hip_kv_store": (i32, [vp, i32, i32, vp, vp]),
     "gllm_hip_kv_store_dev": (i32, [vp, i32, i32, vp, vp, vp]),

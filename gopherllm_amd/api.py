@@ -511,12 +511,16 @@ class KVCacheF16:
 
     def tensors(self, layer):
         """(K, V) of a layer as float16 tensors of max_len rows over the cache's own
-        memory: they hold this object, and end with release() (or, for a decoder's
-        cache, with the decoder)."""
+        memory, on its device: they hold this object, and end with release() (or, for a
+        decoder's cache, with the decoder)."""
         import torch
         if not 0 <= layer < self.layers:
             raise ValueError(f"tensors: layer {layer} of {self.layers}")
-        return tuple(torch.as_tensor(_DeviceRows(self, p, self.max_len, d), device="cuda")
+        if not self.handle:
+            raise ValueError("tensors: the cache is released")
+        # the device by its number: on any other one, the current one too, torch would make a copy
+        device = f"cuda:{load().gllm_hip_kv_device(self.handle)}"
+        return tuple(torch.as_tensor(_DeviceRows(self, p, self.max_len, d), device=device)
                      for p, d in ((self.k_ptr(layer), self.kv_dim_k), (self.v_ptr(layer), self.kv_dim_v)))
 
     def store_rope_dev(self, layer, rope: Rope, q, k, v, positions, rows, q_out=None, stream=None):

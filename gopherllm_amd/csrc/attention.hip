@@ -1719,6 +1719,10 @@ uint16_t* gllm_hip_kv_v_dev(gllm_hip_kv* kv, int l) {
     return kv->v[l];
 }
 
+int gllm_hip_kv_device(const gllm_hip_kv* kv) {
+    return kv ? kv->device : fail(GLLM_EINVAL, "gllm_hip_kv_device: null cache");
+}
+
 int gllm_hip_kv_read(gllm_hip_kv* kv, int l, int pos0, int n, uint16_t* k_out, uint16_t* v_out) {
     if (!kv || l < 0 || l >= kv->layers || pos0 < 0 || n < 0 || pos0 + n > kv->max_len)
         return fail(GLLM_EINVAL, "gllm_hip_kv_read: bad range");

@@ -249,6 +249,8 @@ void gllm_hip_kv_release(gllm_hip_kv* kv);
 /* Device pointer of layer l's K (or V) rows: [max_len][kv_dim] uint16. */
 uint16_t* gllm_hip_kv_k_dev(gllm_hip_kv* kv, int l);
 uint16_t* gllm_hip_kv_v_dev(gllm_hip_kv* kv, int l);
+/* The device that holds them, or GLLM_EINVAL. */
+int gllm_hip_kv_device(const gllm_hip_kv* kv);
 /* Copy n positions starting at pos0 of layer l to host (f16 bits); either
  * output may be NULL.  (The rows a prefix cache would copy, runtime.go:1334.) */
 int gllm_hip_kv_read(gllm_hip_kv* kv, int l, int pos0, int n, uint16_t* k_out, uint16_t* v_out);

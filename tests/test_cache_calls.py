@@ -1,11 +1,13 @@
 """What the cache calls' Python side does before the library is called, with
 stand-ins for torch and its tensors: no device is needed."""
+import ctypes as C
 import sys
 import threading
 import types
 
 import pytest
 
+import gopherllm_amd as g
 from gopherllm_amd import api
 
 
@@ -58,3 +60,42 @@ def test_first_calls_of_two_threads(fresh):
         go.set()
         first.join()
     assert got == [(0, 77)]
+
+
+# --- a layer's rows as tensors -------------------------------------------------
+
+
+class Cache(C.Structure):
+    """csrc/kv_cache.h"""
+    _fields_ = [(n, C.c_int) for n in ("layers", "kv_dim_k", "kv_dim_v", "max_len")] + [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("device", C.c_int)]
+
+
+def cache(device=0, layers=2, kd=256, vd=128, rows=100):
+    """A KVCacheF16 over a handle of our own; its rows' addresses are never read."""
+    at = (C.c_void_p * (2 * layers))(*[4096 * (i + 1) for i in range(2 * layers)])
+    raw = Cache(layers, kd, vd, rows, C.addressof(at), C.addressof(at) + 8 * layers, device)
+    kv = api.KVCacheF16(layers, kd, vd, rows, handle=C.addressof(raw), owned=False)
+    kv.kept = (at, raw)
+    return kv
+
+
+@pytest.mark.parametrize("device", [0, 3])
+def test_tensors_are_on_the_caches_device(monkeypatch, device):
+    """Whatever the current device is: torch copies rows that are asked for on another one."""
+    import torch
+    asked = []
+    monkeypatch.setattr(torch, "as_tensor", lambda rows, device: asked.append((rows.__cuda_array_interface__, str(torch.device(device)))))
+    cache(device).tensors(1)
+    assert [(a["data"][0], a["shape"], d) for a, d in asked] == [(8192, (100, 256), f"cuda:{device}"), (16384, (100, 128), f"cuda:{device}")]
+
+
+def test_tensors_refusals():
+    kv = cache()
+    for layer in (-1, 2):
+        with pytest.raises(ValueError):
+            kv.tensors(layer)
+    kv.release()
+    with pytest.raises(ValueError, match="released"):
+        kv.tensors(0)
+    assert g.load().gllm_hip_kv_device(None) == g.EINVAL

@@ -56,3 +56,17 @@ def test_mass_of_scores_far_from_zero(hip, n, heads, n_kv, hd, start, end, offse
 def test_mass_score_ranges(hip, n, heads, n_kv, hd, start, end, std, scale):
     """Scores from all equal to one row that takes it all, and keys from f16's least subnormals to large ones."""
     check_mass(hip, n, heads, n_kv, hd, start, end, 1100 + n + hd, std=std, scale=scale)
+
+
+def test_tensors_are_the_caches_rows(hip):
+    """Not copies: the addresses are the cache's, and what is written through them is read back from it."""
+    import torch
+    kv = hip.KVCacheF16(2, 24, 40, 9)
+    for l in range(2):
+        k, v = kv.tensors(l)
+        assert (k.data_ptr(), v.data_ptr()) == (kv.k_ptr(l), kv.v_ptr(l)) and k.get_device() == v.get_device() == torch.cuda.current_device()
+        k.fill_(1.5 + l)
+        v.fill_(-2.0 - l)
+        torch.cuda.synchronize()
+        rk, rv = kv.read(l, 0, 9)
+        assert (rk.view(np.float16) == 1.5 + l).all() and (rv.view(np.float16) == -2.0 - l).all()
