@@ -111,12 +111,24 @@ def _ptr_rows(t, kind: str, n: int, dim: int, what: str, at: int):
         shape = (1, shape[0])
     if len(shape) != 2 or shape[0] != n or shape[1] != dim:
         raise ValueError(f"{what}: shape {tuple(t.shape)}, need {n} rows of {dim}")
+    outer = dim
     if not t.is_contiguous():
         inner, outer = t.stride(-1), t.stride(0) if n > 1 else dim
         if dim > 1 and inner != 1 or outer < dim:
             raise ValueError(f"{what}: the values of a row must be contiguous, and rows must not overlap")
-        return t.data_ptr(), outer
-    return t.data_ptr(), dim
+    if (n | outer) >> 31:
+        raise ValueError(f"{what}: {n} rows, {outer} values apart, do not fit 32 bits")
+    return t.data_ptr(), outer
+
+
+def _sizes(what: str, either: int, *values):
+    """The library's whole numbers are 32 bits, and ctypes cuts larger ones without
+    a word.  either: the values or-ed together, which settles the usual case at once;
+    negative ones are the library's to refuse."""
+    if either >> 31:
+        for x in values:
+            if not -(1 << 31) <= x < 1 << 31:
+                raise ValueError(f"{what}: {x} does not fit 32 bits")
 
 
 def _work(work, at):
@@ -385,9 +397,11 @@ class Rope:
                freq_factors=None):
         if layout not in cls.LAYOUTS or scaling not in cls.SCALINGS:
             raise ValueError(f"Rope: layout {layout!r}, scaling {scaling!r}")
+        sizes = int(head_dim), int(head_dim if rot_dim is None else rot_dim), int(orig_ctx)
+        _sizes("Rope", 1 << 31, *sizes)
         c = _lib.RopeConfig()
-        c.head_dim, c.rot_dim = int(head_dim), int(head_dim if rot_dim is None else rot_dim)
-        c.layout, c.scaling, c.orig_ctx = cls.LAYOUTS[layout], cls.SCALINGS[scaling], int(orig_ctx)
+        c.head_dim, c.rot_dim, c.orig_ctx = sizes
+        c.layout, c.scaling = cls.LAYOUTS[layout], cls.SCALINGS[scaling]
         c.theta, c.factor, c.attn_factor = float(theta), float(factor), float(attn_factor)
         c.low_freq_factor, c.high_freq_factor = float(low_freq_factor), float(high_freq_factor)
         c.beta_fast, c.beta_slow = float(beta_fast), float(beta_slow)
@@ -432,16 +446,19 @@ class Rope:
 
 def attend_shared_bytes(n, n_heads, n_kv_heads, hd, length, most) -> int:
     """Bytes of a workspace for KVCacheF16.attend_shared_dev."""
+    _sizes("attend_shared_bytes", n | n_heads | n_kv_heads | hd | length | most, n, n_heads, n_kv_heads, hd, length, most)
     return int(load().gllm_hip_attend_shared_bytes(n, n_heads, n_kv_heads, hd, length, most))
 
 
 def attend_mass_bytes(n, n_heads, n_kv_heads, hd, length) -> int:
     """Bytes of a workspace for KVCacheF16.attend_mass_dev over `length` rows."""
+    _sizes("attend_mass_bytes", n | n_heads | n_kv_heads | hd | length, n, n_heads, n_kv_heads, hd, length)
     return int(load().gllm_hip_attend_mass_bytes(n, n_heads, n_kv_heads, hd, length))
 
 
 def keep_bytes(layers, n_kv_heads, budget) -> int:
     """Bytes of a workspace for KVCacheF16.keep_dev."""
+    _sizes("keep_bytes", layers | n_kv_heads | budget, layers, n_kv_heads, budget)
     return int(load().gllm_hip_kv_keep_bytes(layers, n_kv_heads, budget))
 
 
@@ -533,6 +550,7 @@ class KVCacheF16:
         heads, n_kv = qd // hd, kd // hd
         if kd != n_kv * hd or qd != heads * hd:
             raise ValueError(f"store_rope_dev: q or k rows are not heads of {hd}")
+        _sizes("store_rope_dev", layer, layer)
         qp = op = None
         qs = os = 0
         if q is not None:
@@ -553,6 +571,8 @@ class KVCacheF16:
         at, current = _here()
         n = q.shape[0] if q.dim() > 1 else 1
         numel = n * n_heads * hd
+        _sizes("attend_shared_dev", layer | n | n_heads | n_kv_heads | hd | start | length | most,
+               layer, n, n_heads, n_kv_heads, hd, start, length, most)
         wp, wb = _work(work, at)
         call("gllm_hip_attend_shared_dev", self.handle, layer, _ptr(q, "f32", numel, "q", at), n, n_heads, n_kv_heads,
              hd, start, length, None if starts is None else _ptr(starts, "i32", n, "starts", at),
@@ -566,6 +586,8 @@ class KVCacheF16:
         at, current = _here()
         n = q.shape[0] if q.dim() > 1 else 1
         numel, stride = n * n_heads * hd, mass.shape[-1]
+        _sizes("attend_mass_dev", layer | n | n_heads | n_kv_heads | hd | start | end | stride,
+               layer, n, n_heads, n_kv_heads, hd, start, end, stride)
         wp, wb = _work(work, at)
         call("gllm_hip_attend_mass_dev", self.handle, layer, _ptr(q, "f32", numel, "q", at), n, n_heads, n_kv_heads, hd,
              start, end, scale, _ptr(mass, "f32", n_kv_heads * stride, "mass", at), stride,
@@ -583,6 +605,8 @@ class KVCacheF16:
         if pos is not None and pos.shape[-1] != stride or pos_out.shape[-1] != out_stride:
             raise ValueError("keep_dev: mass and pos rows of different lengths")
         n = self.layers * n_kv_heads
+        _sizes("keep_dev", n_kv_heads | hd | start | length | dst_start | budget | sinks | recent | now | stride | out_stride,
+               n_kv_heads, hd, start, length, dst_start, budget, sinks, recent, now, stride, out_stride)
         wp, wb = _work(work, at)
         call("gllm_hip_kv_keep_dev", self.handle, dst.handle, n_kv_heads, hd, start, length, dst_start, budget, sinks,
              recent, now, _ptr(mass, "f32", n * stride, "mass", at),
@@ -600,6 +624,8 @@ class KVCacheF16:
         stride, dim = mass.shape[-1], n_kv_heads * hd
         if pos.shape[-1] != stride:
             raise ValueError("evict_store_dev: mass and pos rows of different lengths")
+        _sizes("evict_store_dev", layer | n_kv_heads | hd | start | length | sinks | recent | stride,
+               layer, n_kv_heads, hd, start, length, sinks, recent, stride)
         call("gllm_hip_kv_evict_store_dev", self.handle, layer, n_kv_heads, hd, _ptr(k, "f32", dim, "k", at),
              _ptr(v, "f32", dim, "v", at), start, length, sinks, recent,
              _ptr(mass, "f32", n_kv_heads * stride, "mass", at), _ptr(pos, "i32", n_kv_heads * stride, "pos", at), stride,

@@ -5,6 +5,7 @@ import sys
 import threading
 import types
 
+import numpy as np
 import pytest
 
 import gopherllm_amd as g
@@ -99,3 +100,129 @@ def test_tensors_refusals():
     with pytest.raises(ValueError, match="released"):
         kv.tensors(0)
     assert g.load().gllm_hip_kv_device(None) == g.EINVAL
+
+
+# --- sizes and strides past 32 bits, which ctypes would cut ----------------------
+
+
+class Tensor:
+    """A device tensor as the calls look at it: shape and strides without memory."""
+
+    def __init__(self, *shape, kind="float32", strides=None, device=0):
+        self.shape, self.dtype, self.device, self.is_cuda = shape, kind, device, True
+        self.strides = strides or [int(np.prod(shape[i + 1:], dtype=np.int64)) for i in range(len(shape))]
+        self.whole = strides is None
+
+    def stride(self, i):
+        return self.strides[i]
+
+    def get_device(self):
+        return self.device
+
+    def numel(self):
+        return int(np.prod(self.shape, dtype=np.int64))
+
+    def dim(self):
+        return len(self.shape)
+
+    def is_contiguous(self):
+        return self.whole
+
+    def data_ptr(self):
+        return 4096
+
+
+def ints(*shape):
+    return Tensor(*shape, kind="int32")
+
+
+@pytest.fixture
+def calls(fresh, monkeypatch):
+    """The library calls that get through, with their arguments."""
+    fresh(Torch())
+    got = []
+    monkeypatch.setattr(api, "call", lambda name, *args: got.append((name, *args)))
+    return got
+
+
+def rope(hd=64):
+    r = object.__new__(api.Rope)
+    r.handle, r.head_dim = None, hd
+    return r
+
+
+FAR = (1 << 32) + 128  # 128 when it is cut
+SHARED = dict(layer=0, q=Tensor(3, 512), n_heads=8, n_kv_heads=2, hd=64, start=0, length=10, starts=ints(3), lens=ints(3), most=4,
+              scale=0.1, out=Tensor(3, 512))
+MASS = dict(layer=0, q=Tensor(3, 512), n_heads=8, n_kv_heads=2, hd=64, start=0, end=9, scale=0.1, mass=Tensor(2, 100), out=Tensor(3, 512))
+KEEP = dict(n_kv_heads=2, hd=64, length=50, budget=20, mass=Tensor(2, 2, 100), pos=ints(2, 2, 100), mass_out=Tensor(2, 2, 30),
+            pos_out=ints(2, 2, 30), now=50)
+EVICT = dict(layer=0, n_kv_heads=2, hd=64, k=Tensor(128), v=Tensor(128), start=0, length=50, mass=Tensor(2, 100), pos=ints(2, 100), now=ints(1))
+
+
+@pytest.mark.parametrize("name,args,changed", [("attend_shared_dev", SHARED, dict(a)) for a in [
+    dict(layer=FAR), dict(start=FAR), dict(length=FAR), dict(most=FAR), dict(start=-FAR), dict(length=-(1 << 32))]] +
+    [("attend_mass_dev", MASS, dict(a)) for a in [dict(start=FAR), dict(end=FAR), dict(layer=FAR), dict(mass=Tensor(2, FAR))]] +
+    [("keep_dev", KEEP, dict(a)) for a in [
+        dict(length=FAR), dict(budget=FAR), dict(now=FAR), dict(sinks=1 << 32), dict(recent=1 << 40), dict(start=FAR), dict(dst_start=FAR),
+        dict(mass=Tensor(2, 2, FAR), pos=None), dict(mass_out=Tensor(2, 2, FAR), pos_out=ints(2, 2, FAR))]] +
+    [("evict_store_dev", EVICT, dict(a)) for a in [
+        dict(length=FAR), dict(sinks=1 << 32), dict(recent=1 << 40), dict(start=FAR), dict(layer=FAR),
+        dict(mass=Tensor(2, FAR), pos=ints(2, FAR))]])
+def test_sizes_past_32_bits_are_refused(calls, name, args, changed):
+    kv = cache()
+    lead = (cache(rows=30),) if name == "keep_dev" else ()
+    getattr(kv, name)(*lead, **args)
+    assert len(calls) == 1  # as it is, the call gets through
+    with pytest.raises(ValueError):
+        getattr(kv, name)(*lead, **{**args, **changed})
+    assert len(calls) == 1
+
+
+def test_a_layer_past_32_bits_is_refused(calls):
+    args = dict(rope=rope(), q=None, k=Tensor(3, 128), v=Tensor(3, 128), positions=ints(3), rows=ints(3))
+    with pytest.raises(ValueError, match="32"):
+        cache().store_rope_dev(1 << 32, **args)
+    assert not calls
+
+
+def test_negative_sizes_are_the_librarys_to_refuse(calls):
+    cache().attend_shared_dev(**{**SHARED, "start": -1, "length": -5})
+    assert calls[0][8:10] == (-1, -5)
+
+
+@pytest.mark.parametrize("which", ["q", "k", "v", "q_out"])
+def test_row_strides_past_32_bits_are_refused(calls, which):
+    kv, n, d = cache(), 3, 128
+    args = dict(q=Tensor(n, d), k=Tensor(n, d), v=Tensor(n, d), positions=ints(n), rows=ints(n), q_out=Tensor(n, d))
+    wide = {**args, which: Tensor(n, d, strides=[(1 << 31) - 1, 1])}
+    kv.store_rope_dev(0, rope(), **wide)
+    assert len(calls) == 1 and (1 << 31) - 1 in calls[0]
+    for stride in (1 << 31, FAR):
+        with pytest.raises(ValueError, match="32"):
+            kv.store_rope_dev(0, rope(), **{**args, which: Tensor(n, d, strides=[stride, 1])})
+        with pytest.raises(ValueError, match="32"):
+            rope().apply_dev(Tensor(n, d, strides=[stride, 1]), ints(n), Tensor(n, d))
+    assert len(calls) == 1
+
+
+def test_more_tokens_than_32_bits_count_are_refused(calls):
+    n = (1 << 32) + 1
+    with pytest.raises(ValueError, match="32"):
+        rope().apply_dev(Tensor(n, 128), ints(n), Tensor(n, 128))
+    with pytest.raises(ValueError, match="32"):
+        cache().attend_shared_dev(**{**SHARED, "q": Tensor(n, 512), "out": Tensor(n, 512), "starts": ints(n), "lens": ints(n)})
+    assert not calls
+
+
+@pytest.mark.parametrize("kw", [dict(head_dim=FAR), dict(head_dim=128, rot_dim=FAR), dict(head_dim=128, orig_ctx=FAR)])
+def test_rope_sizes_past_32_bits_are_refused(kw):
+    with pytest.raises(ValueError, match="32"):
+        g.Rope.config(**kw)
+
+
+@pytest.mark.parametrize("name,args", [("attend_shared_bytes", (4, 8, 2, 64, FAR, 4)), ("attend_shared_bytes", (4, 8, 2, 64, 10, FAR)),
+                                       ("attend_mass_bytes", (4, 8, 2, 64, FAR)), ("keep_bytes", (4, 8, FAR))])
+def test_workspaces_past_32_bits_are_refused(name, args):
+    with pytest.raises(ValueError, match="32"):
+        getattr(g, name)(*args)
