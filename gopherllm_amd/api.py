@@ -131,6 +131,16 @@ def _sizes(what: str, either: int, *values):
                 raise ValueError(f"{what}: {x} does not fit 32 bits")
 
 
+def _ptr_tokens(t, n: int, dim: int, what: str, at: int):
+    """Pointer of n rows of dim float32 values, one after the other; more rows may follow."""
+    if t.numel() == n * dim and t.dtype in _kinds["f32"] and t.get_device() == at and t.is_contiguous():
+        return t.data_ptr()
+    p = _ptr(t, "f32", n * dim, what, at)
+    if t.dim() > 1 and t.numel() != t.shape[0] * dim:
+        raise ValueError(f"{what}: shape {tuple(t.shape)}, need {n} rows of {dim}")
+    return p
+
+
 def _work(work, at):
     """(pointer, bytes) of a caller's workspace, or of none."""
     if work is None:
@@ -569,29 +579,27 @@ class KVCacheF16:
         start .. start + length - 1 and, with most > 0, its own lens[i] rows from
         starts[i] (int32 tensors; most: the length the work is split for)."""
         at, current = _here()
-        n = q.shape[0] if q.dim() > 1 else 1
-        numel = n * n_heads * hd
+        n, dim = q.shape[0] if q.dim() > 1 else 1, n_heads * hd
         _sizes("attend_shared_dev", layer | n | n_heads | n_kv_heads | hd | start | length | most,
                layer, n, n_heads, n_kv_heads, hd, start, length, most)
         wp, wb = _work(work, at)
-        call("gllm_hip_attend_shared_dev", self.handle, layer, _ptr(q, "f32", numel, "q", at), n, n_heads, n_kv_heads,
+        call("gllm_hip_attend_shared_dev", self.handle, layer, _ptr_tokens(q, n, dim, "q", at), n, n_heads, n_kv_heads,
              hd, start, length, None if starts is None else _ptr(starts, "i32", n, "starts", at),
              None if lens is None else _ptr(lens, "i32", n, "lens", at), most, scale,
-             _ptr(out, "f32", numel, "out", at), wp, wb, current if stream is None else stream)
+             _ptr_tokens(out, n, dim, "out", at), wp, wb, current if stream is None else stream)
         return out
 
     def attend_mass_dev(self, layer, q, n_heads, n_kv_heads, hd, start, end, scale, mass, out, work=None, stream=None):
         """The newest tokens q (tokens, n_heads * hd), the last at row `end`, causally over
         rows start .. end; each row's weight is added to mass (n_kv_heads, >= end + 1)."""
         at, current = _here()
-        n = q.shape[0] if q.dim() > 1 else 1
-        numel, stride = n * n_heads * hd, mass.shape[-1]
+        n, dim, stride = q.shape[0] if q.dim() > 1 else 1, n_heads * hd, mass.shape[-1]
         _sizes("attend_mass_dev", layer | n | n_heads | n_kv_heads | hd | start | end | stride,
                layer, n, n_heads, n_kv_heads, hd, start, end, stride)
         wp, wb = _work(work, at)
-        call("gllm_hip_attend_mass_dev", self.handle, layer, _ptr(q, "f32", numel, "q", at), n, n_heads, n_kv_heads, hd,
+        call("gllm_hip_attend_mass_dev", self.handle, layer, _ptr_tokens(q, n, dim, "q", at), n, n_heads, n_kv_heads, hd,
              start, end, scale, _ptr(mass, "f32", n_kv_heads * stride, "mass", at), stride,
-             _ptr(out, "f32", numel, "out", at), wp, wb, current if stream is None else stream)
+             _ptr_tokens(out, n, dim, "out", at), wp, wb, current if stream is None else stream)
         return out
 
     def keep_dev(self, dst: "KVCacheF16", n_kv_heads, hd, length, budget, mass, pos, mass_out, pos_out, now, sinks=0,

@@ -226,3 +226,22 @@ def test_rope_sizes_past_32_bits_are_refused(kw):
 def test_workspaces_past_32_bits_are_refused(name, args):
     with pytest.raises(ValueError, match="32"):
         getattr(g, name)(*args)
+
+
+# --- rows of another width ----------------------------------------------------
+
+
+@pytest.mark.parametrize("name,args", [("attend_shared_dev", SHARED), ("attend_mass_dev", MASS)])
+def test_rows_of_another_width_are_refused(calls, name, args):
+    """Tokens are read and written n_heads * hd apart: wider rows, such as a fused projection's, are not."""
+    kv = cache()
+    for wrong in (dict(q=Tensor(3, 768)), dict(q=Tensor(3, 2, 512)), dict(out=Tensor(3, 768)), dict(out=Tensor(4, 520)), dict(out=Tensor(3, 511))):
+        with pytest.raises(ValueError):
+            getattr(kv, name)(**{**args, **wrong})
+    assert not calls
+    right = [dict(q=Tensor(3, 8, 64)), dict(out=Tensor(3, 8, 64)), dict(out=Tensor(5, 512)), dict(out=Tensor(4000)), dict(out=Tensor(24, 64))]
+    if name == "attend_shared_dev":
+        right.append(dict(q=Tensor(512), starts=ints(1), lens=ints(1), out=Tensor(8, 64)))
+    for also in right:
+        getattr(kv, name)(**{**args, **also})
+    assert len(calls) == len(right)
