@@ -727,6 +727,14 @@ static void seq_launch_hd(const SeqArgs& a, int blocks, hipStream_t s) {
     else hipLaunchKernelGGL((seq_attend_kernel<128, NQ, RW>), dim3(blocks), dim3(256), 0, s, a);
 }
 
+constexpr int kSeqMaxLen = 1 << 30;  // rows of a cache
+
+// Sizes that seq_check takes, for the workspaces
+static bool seq_sizes(int n, int n_heads, int n_kv, int hd, int len) {
+    return n >= 1 && n_kv >= 1 && n_heads >= 1 && n_heads % n_kv == 0 && hd >= 8 && hd % 8 == 0 && hd <= 128 && len >= 0 &&
+           len <= kSeqMaxLen && (long long)n * n_heads <= kSeqMaxRows;
+}
+
 static int seq_check(const char* what, const gllm_hip_kv* kv, int l, const float* d_q, int n, int n_heads, int n_kv,
                      int hd, const float* d_out) {
     if (n < 1) return fail(GLLM_EINVAL, "%s: %d tokens", what, n);
@@ -737,7 +745,7 @@ static int seq_check(const char* what, const gllm_hip_kv* kv, int l, const float
     if (l < 0 || l >= kv->layers) return fail(GLLM_EINVAL, "%s: layer %d out of range", what, l);
     if ((long long)n_kv * hd > kv->kv_dim_k || (long long)n_kv * hd > kv->kv_dim_v)
         return fail(GLLM_EINVAL, "%s: %d kv heads of %d do not fit the cache", what, n_kv, hd);
-    if (kv->max_len > 1 << 30 || kv->kv_dim_k > 1 << 24 || kv->kv_dim_v > 1 << 24)
+    if (kv->max_len > kSeqMaxLen || kv->kv_dim_k > 1 << 24 || kv->kv_dim_v > 1 << 24)
         return fail(GLLM_EUNSUP, "%s: a cache of %d rows of %d and %d values", what, kv->max_len, kv->kv_dim_k, kv->kv_dim_v);
     if (kv->kv_dim_k % 8 || kv->kv_dim_v % 8)
         return fail(GLLM_EUNSUP, "%s: cache rows of %d and %d values are not 16-byte aligned", what, kv->kv_dim_k, kv->kv_dim_v);
@@ -821,9 +829,7 @@ using namespace gllm;
 extern "C" {
 
 size_t gllm_hip_attend_shared_bytes(int n, int n_heads, int n_kv_heads, int hd, int len, int most) {
-    if (n < 1 || n_kv_heads < 1 || n_heads < 1 || n_heads % n_kv_heads || hd < 1 || hd > 128 || len < 0 || most < 0 ||
-        (long long)n * n_heads > kSeqMaxRows)
-        return 0;
+    if (!seq_sizes(n, n_heads, n_kv_heads, hd, len) || most < 0) return 0;
     return 4 * seq_floats(seq_plan(n, n_heads, n_kv_heads, hd, len, most), hd);
 }
 
@@ -852,9 +858,7 @@ int gllm_hip_attend_shared_dev(gllm_hip_kv* kv, int l, const float* d_q, int n, 
 }
 
 size_t gllm_hip_attend_mass_bytes(int n, int n_heads, int n_kv_heads, int hd, int len) {
-    if (n < 1 || n_kv_heads < 1 || n_heads < 1 || n_heads % n_kv_heads || hd < 1 || hd > 128 || len < 1 ||
-        n > len || (long long)n * n_heads > kSeqMaxRows)
-        return 0;
+    if (!seq_sizes(n, n_heads, n_kv_heads, hd, len) || n > len) return 0;
     return 4 * mass_floats(seq_plan(n, n_heads, n_kv_heads, hd, len - (n - 1), n - 1), hd, n_kv_heads, len);
 }
 

@@ -245,3 +245,18 @@ def test_rows_of_another_width_are_refused(calls, name, args):
     for also in right:
         getattr(kv, name)(**{**args, **also})
     assert len(calls) == len(right)
+
+
+# --- workspaces -----------------------------------------------------------------
+
+
+def test_no_workspace_for_sizes_that_a_call_refuses():
+    """Longer than a cache can be, and head sizes that attention does not take."""
+    far = 1 << 30
+    for n_kv in (1, 512, 4096):
+        assert g.attend_shared_bytes(1, n_kv, n_kv, 8, far, 0) > 0 and g.attend_mass_bytes(1, n_kv, n_kv, 8, far) >= 4 * n_kv * far
+        for length in (far + 1, 2**31 - 1):
+            assert g.attend_shared_bytes(1, n_kv, n_kv, 8, length, 0) == 0 and g.attend_mass_bytes(1, n_kv, n_kv, 8, length) == 0
+    for hd in (0, 1, 7, 12, 127, 136):
+        assert g.attend_shared_bytes(2, 4, 2, hd, 10, 3) == 0 and g.attend_mass_bytes(2, 4, 2, hd, 10) == 0
+    assert g.attend_shared_bytes(2, 4, 2, 64, 10, 2**31 - 1) > 0  # a plan longer than any cache is still one
