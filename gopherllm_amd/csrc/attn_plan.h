@@ -22,9 +22,36 @@ struct SeqPlan {
     int own_blocks, splits;   // of each token's own range (16 rows a block)
     int slots;                // partial results of a query row
     size_t rows;              // n * n_heads
+    size_t parts;             // partial results that the workspace has room for
 };
 
 inline int ceil_div(int a, int b) { return (int)(((long long)a + b - 1) / b); }
+
+inline bool seq_much(long long per_kv, int n_kv, int hd, int len) { return per_kv * (double)len * n_kv * hd > 4.0e9; }
+
+// Room for rows x slots partial results that never falls as n, len or most grow,
+// so a workspace for the most of each serves every smaller call (the slots
+// themselves fall where a chunk grows by a step: 64 over 8192 positions, 33 over
+// 8193).  A row has at most 64 and one for each 128 positions of either range, and
+//   shared  n_kv * row_blocks * chunks <= kSeqTarget, or one chunk, with row_blocks
+//           of at most 16 nq rw of a kv head's rows (nq as for the largest head)
+//   own     n * n_kv * own_blocks * splits <= kSeqTarget, or one split
+inline size_t seq_parts(int n, int n_heads, int n_kv, int len, int most) {
+    const size_t rows = (size_t)n * n_heads;
+    const int r = n_heads / n_kv;
+    const long long per_kv = (long long)n * r;
+    const auto cap = [&](int positions) { return rows * std::min(kSeqMaxSplits, ceil_div(positions, kSeqQuantum)); };
+    size_t parts = 0;
+    if (len > 0) {
+        const size_t block = per_kv <= 16 ? 16 : per_kv > 64 && seq_much(per_kv, n_kv, 128, len) ? 32 * kSeqWaves : 16 * kSeqWaves;
+        parts += std::min(cap(len), std::max(rows, kSeqTarget * block));
+    }
+    if (most > 0) {
+        const size_t own_blocks = ceil_div(r, 16);
+        parts += std::min(cap(most), std::max(rows, ((size_t)kSeqTarget * r + own_blocks - 1) / own_blocks));
+    }
+    return parts;
+}
 
 // n tokens, heads / kv heads of hd, `len` shared positions, own ranges planned for
 // `most` positions (0: none).
@@ -41,7 +68,7 @@ inline SeqPlan seq_plan(int n, int n_heads, int n_kv, int hd, int len, int most)
     // 128 x 8000 22 and 28.
     p.rw = per_kv <= 16 ? 1 : kSeqWaves;
     const bool fits = (per_kv + 63) / 64 * 64 == (per_kv + 127) / 128 * 128;
-    p.nq = fits && per_kv * (double)len * n_kv * hd > 4.0e9 ? 2 : 1;
+    p.nq = fits && seq_much(per_kv, n_kv, hd, len) ? 2 : 1;
     p.row_blocks = (int)((per_kv + 16 * p.nq * p.rw - 1) / (16 * p.nq * p.rw));
     if (len > 0) {
         const long long per_chunk = (long long)n_kv * p.row_blocks;
@@ -64,11 +91,12 @@ inline SeqPlan seq_plan(int n, int n_heads, int n_kv, int hd, int len, int most)
         p.splits = std::min(want, ceil_div(most, kSeqQuantum));
     }
     p.slots = p.chunks + p.splits;
+    p.parts = seq_parts(n, n_heads, n_kv, len, most);
     return p;
 }
 
 // Floats of the partial results: base and sum of each, and its output.
-inline size_t seq_floats(const SeqPlan& p, int hd) { return p.rows * (size_t)p.slots * (2 + (size_t)hd) + 64; }
+inline size_t seq_floats(const SeqPlan& p, int hd) { return p.parts * (2 + (size_t)hd) + 64; }
 
 // What attention with weights works in, in floats: one token's query rows (up to
 // 16 a kv head) keep their scores, more keep their operands (f16 pairs, in the matrix cores' order),
@@ -94,7 +122,14 @@ inline MassSpace mass_space(const SeqPlan& p, int hd, int n_kv, int len) {
     }
     return m;
 }
-inline size_t mass_floats(const SeqPlan& p, int hd, int n_kv, int len) { return mass_space(p, hd, n_kv, len).parts + seq_floats(p, hd); }
+
+// Floats of it with the partial results: like seq_parts, as many as any call of
+// fewer tokens over fewer positions needs, one token's kept scores among them.
+inline size_t mass_floats(const SeqPlan& p, int hd, int n_kv, int len) {
+    const int n_heads = p.r * n_kv, n = (int)(p.rows / n_heads);
+    const size_t one = p.r <= 16 ? n_heads * (((size_t)len + 3) / 4 * 4) : 0;
+    return std::max(mass_space(p, hd, n_kv, len).parts, one) + seq_parts(n, n_heads, n_kv, len, n - 1) * (2 + (size_t)hd) + 64;
+}
 
 // Rows a .. b - 1 of a cache of max_len rows that the range start, len names.
 struct RowSpan {

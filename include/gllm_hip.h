@@ -280,7 +280,9 @@ int gllm_hip_attend_dev(gllm_hip_kv* kv, int l, const float* d_q, int n_heads, i
 /* Workspaces: a call that takes d_work / work_bytes works in that device   */
 /* buffer (16-byte aligned, at least the bytes its _bytes function says,   */
 /* which says 0 of sizes that the call refuses), or, with d_work null, in  */
-/* the calling thread's scratch for the stream.                            */
+/* the calling thread's scratch for the stream.  Those bytes never fall as */
+/* tokens, lengths or budgets grow: what serves the largest call of a run  */
+/* serves all of them.                                                     */
 /* Graphs captured on one stream with null share that scratch and must not */
 /* be replayed at the same time; with a d_work each they may.  Caches,      */
 /* ropes and tensors must be on the current device (GLLM_EINVAL).          */

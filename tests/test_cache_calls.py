@@ -260,3 +260,34 @@ def test_no_workspace_for_sizes_that_a_call_refuses():
     for hd in (0, 1, 7, 12, 127, 136):
         assert g.attend_shared_bytes(2, 4, 2, hd, 10, 3) == 0 and g.attend_mass_bytes(2, 4, 2, hd, 10) == 0
     assert g.attend_shared_bytes(2, 4, 2, 64, 10, 2**31 - 1) > 0  # a plan longer than any cache is still one
+
+
+HEADS = [(32, 8, 128), (8, 2, 64), (40, 8, 80), (71, 1, 128), (16, 16, 8), (3, 1, 24)]
+
+
+@pytest.mark.parametrize("heads,n_kv,hd", HEADS)
+def test_workspaces_never_fall(heads, n_kv, hd):
+    """One workspace, sized for the most tokens and the longest ranges, serves every smaller call."""
+    ns = [1, 2, 3, 4, 5, 8, 9, 16, 17, 32, 33, 63, 64, 65, 128, 256, 300, 1024, 4096]
+    lens = [0, 1, 31, 127, 128, 129, 300, 640, 1000, 2049, 4001, 4096, 5000, 8192, 8193, 16001, 32768, 50000, 131072, 1 << 20, 1 << 30]
+    mosts = [0, 1, 17, 128, 129, 640, 1024, 4096, 8193, 1 << 20, 2**31 - 1]
+    size = {(n, a, b): g.attend_shared_bytes(n, heads, n_kv, hd, a, b) for n in ns for a in lens for b in mosts}
+    for (n, a, b), x in size.items():
+        for other in ((m, a, b) for m in ns[:ns.index(n)][-1:]), ((n, m, b) for m in lens[:lens.index(a)][-1:]), ((n, a, m) for m in mosts[:mosts.index(b)][-1:]):
+            for o in other:
+                assert size[o] <= x, (o, (n, a, b))
+    mass = {(n, a): g.attend_mass_bytes(n, heads, n_kv, hd, a) for n in ns for a in lens if n <= a}
+    for (n, a), x in mass.items():
+        assert all(mass[n, m] <= x for m in lens if n <= m < a), (n, a)
+        assert all(mass[m, a] <= x for m in ns if m < n), (n, a)
+    # and they stay within twice the partial results of the largest grid
+    assert size[64, 32768, 1024] <= 4 * (2 + hd) * 2 * (64 * heads + 65536 + 512 * heads // n_kv) + 256
+    assert [g.keep_bytes(3, n_kv, b) for b in (1, 5, 700)] == sorted(g.keep_bytes(3, n_kv, b) for b in (1, 5, 700))
+
+
+def test_every_length_fits_the_longest_ones_workspace():
+    for n, most in ((1, 0), (8, 640), (33, 200), (64, 1024)):
+        sizes = [g.attend_shared_bytes(n, 32, 8, 128, length, most) for length in range(0, 9000, 7)]
+        assert sizes == sorted(sizes)
+        sizes = [g.attend_mass_bytes(n, 32, 8, 128, length) for length in range(n, 9000, 7)]
+        assert sizes == sorted(sizes)
