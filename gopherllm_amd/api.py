@@ -145,7 +145,7 @@ def _work(work, at):
     """(pointer, bytes) of a caller's workspace, or of none."""
     if work is None:
         return None, 0
-    return _ptr(work, "u8", 0, "work", at), work.numel()
+    return _ptr(work, "u8", 1, "work", at), work.numel()
 
 
 def _rows(t):

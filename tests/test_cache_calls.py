@@ -291,3 +291,18 @@ def test_every_length_fits_the_longest_ones_workspace():
         assert sizes == sorted(sizes)
         sizes = [g.attend_mass_bytes(n, 32, 8, 128, length) for length in range(n, 9000, 7)]
         assert sizes == sorted(sizes)
+
+
+def test_an_empty_workspace_is_refused(calls):
+    """Its null address would stand for the library's own scratch, which graphs share."""
+    class Empty(Tensor):
+        def data_ptr(self):
+            return 0
+
+    for name, args in (("attend_shared_dev", SHARED), ("attend_mass_dev", MASS), ("keep_dev", KEEP)):
+        lead = (cache(rows=30),) if name == "keep_dev" else ()
+        with pytest.raises(ValueError, match="work"):
+            getattr(cache(), name)(*lead, **args, work=Empty(0, kind="uint8"))
+        assert not calls
+        getattr(cache(), name)(*lead, **args, work=Tensor(64, kind="uint8"))
+        assert calls.pop()[-3:] == (4096, 64, 77)
