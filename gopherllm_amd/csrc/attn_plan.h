@@ -63,29 +63,40 @@ inline SeqPlan seq_plan(int n, int n_heads, int n_kv, int hd, int len, int most)
     // Up to 16 rows: the waves split positions.  More: they share the positions,
     // 16 rows each, or 32 where that leaves no more padding and there is work
     // enough that reading the tiles half as often counts.  With 16 and 32 rows, 8
-    // kv heads of 128, rows x positions: 256 x 32768 81 and 73 us, 1024 x 4000 59
-    // and 54, 256 x 16000 50 and 51, 128 x 32768 48 and 49, 256 x 8000 33 and 36,
-    // 128 x 8000 22 and 28.
+    // kv heads of 128, rows x positions: 256 x 32768 79 and 74 us, 1024 x 4000 59
+    // and 54, 256 x 16000 45.1 and 45.5, 256 x 8000 29 and 33, 128 x 8000 22 and
+    // 28; 8 of 80: 640 x 10000 56 and 54, 640 x 4000 33 and 35; 2 of 64: 1024 x
+    // 32768 55 and 52, 1024 x 8000 24 and 28; one of 128: 2048 x 64000 147 and 131,
+    // 2048 x 16000 46.3 and 46.9, 2048 x 4000 26 and 28; 4 of 32: 2048 x 16000 72
+    // and 59, 2048 x 4000 28.9 and 28.4.
     p.rw = per_kv <= 16 ? 1 : kSeqWaves;
     const bool fits = (per_kv + 63) / 64 * 64 == (per_kv + 127) / 128 * 128;
     p.nq = fits && seq_much(per_kv, n_kv, hd, len) ? 2 : 1;
     p.row_blocks = (int)((per_kv + 16 * p.nq * p.rw - 1) / (16 * p.nq * p.rw));
     if (len > 0) {
         const long long per_chunk = (long long)n_kv * p.row_blocks;
+        const auto chunks = [&](int target) { return (int)std::max(1LL, std::min((long long)kSeqMaxSplits, target / per_chunk)); };
         // Many rows of a shared range keep the matrix cores busy and the own
-        // ranges memory: where these are as long, half the workgroups leave room
-        // for both on a CU (64 requests over 32768 rows and up to 1024 of their
-        // own: 120 us with 512, 114 with 256; without own ranges 78 and 89).
-        const int target = p.rw > 1 && (long long)n * most >= len ? kSeqTarget / 2 : kSeqTarget;
-        const int want = (int)std::max(1LL, std::min((long long)kSeqMaxSplits, target / per_chunk));
+        // ranges memory: where these are planned as long, half the shared workgroups
+        // leave room for both on a CU that holds two of them, as it does for heads
+        // past 96 (64 requests of 32 / 8 heads of 128 over 32768 rows and 513 of
+        // their own: 98 us with 512, 92 with 256; while those are one row, 81 and
+        // 84).  For smaller heads three or four fit (64 of 80: 87 and 112 us; of 64:
+        // 51 and 61), and there only chunks of a few steps do better halved (64 of
+        // 96 over 2000 rows: 22 and 18).
+        int want = chunks(kSeqTarget);
+        if (p.rw > 1 && (long long)n * most >= len && (hd > 96 || ceil_div(len, want) <= kSeqQuantum)) want = chunks(kSeqTarget / 2);
         p.chunk = ceil_div(ceil_div(len, want), kSeqQuantum) * kSeqQuantum;
         p.chunks = ceil_div(len, p.chunk);
     }
     if (most > 0) {
         p.own_blocks = ceil_div(p.r, 16);
         const long long per_split = (long long)n * n_kv * p.own_blocks;
-        // beside the shared range's workgroups, so that all start at once (8 requests
-        // over 4001 rows and up to 640 of their own: 16.3 us with 320 own ones, 14.9 with 256)
+        // as many as the shared range's workgroups leave, and kSeqTarget / 4 at least
+        // (8 requests over 4001 rows and up to 640 of their own: 16.3 us with 320
+        // workgroups for these, 14.9 with the 256 that are left).  More tokens x kv
+        // heads than that wait for shared ones to end: 33 requests of 8 kv heads
+        // are 264 beside 480, 64 are 512 beside 256.
         const int left = std::max(kSeqTarget - n_kv * p.row_blocks * p.chunks, kSeqTarget / 4);
         const int want = (int)std::max(1LL, std::min((long long)kSeqMaxSplits, left / per_split));
         p.splits = std::min(want, ceil_div(most, kSeqQuantum));

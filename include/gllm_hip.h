@@ -334,8 +334,9 @@ int gllm_hip_kv_store_rope_dev(gllm_hip_kv* kv, int l, const gllm_hip_rope* r, c
  * attends the shared rows start .. start + len - 1, read once for the whole
  * batch, and its own rows d_starts[i] .. d_starts[i] + d_lens[i] - 1 (device
  * arrays, cut to the cache; a length <= 0 is none).  `most` is the own length
- * that the work is split for; longer ranges are attended whole too.  most 0
- * with null arrays: no own rows, as for cross attention to an encoder's
+ * that the work is split for; longer ranges are attended whole too, and where
+ * all are far shorter, as early in a captured run, the shared range may have
+ * fewer workgroups than it could (up to a tenth slower).  most 0 with null arrays: no own rows, as for cross attention to an encoder's
  * states.  Ranges may overlap: several tokens of one request are several
  * requests whose own ranges start together (a row in both ranges counts
  * twice).  A request without any row gets zeros.  Sums are float32; q and the
