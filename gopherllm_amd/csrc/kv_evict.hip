@@ -186,7 +186,8 @@ __global__ __launch_bounds__(kKeepThreads) void keep_select_kernel(KeepArgs a) {
             const int before = at_done + at_it[i * kKeepWaves + wave] + __popcll(__ballot(eq) & below);
             if (gt || (eq && before < left)) {
                 const int at = done + up + min(before, left) - min(at_done, left);
-                a.list[lg * a.budget + at] = a.start + t;  // the copy brings its mass and position
+                // always below the budget, unless another stream changes the weights meanwhile
+                if (at < a.budget) a.list[lg * a.budget + at] = a.start + t;  // the copy brings its mass and position
             }
         }
         done += up_all + min(at_done + at_all, left) - min(at_done, left);
@@ -210,7 +211,8 @@ __global__ __launch_bounds__(256) void keep_copy_kernel(KeepPtrs p, KeepArgs a, 
     if (e >= (long long)a.budget * a.n_kv * ch) return;
     const int c = (int)(e % ch), g = (int)(e / ch % a.n_kv), j = (int)(e / ch / a.n_kv);
     const size_t lg = (size_t)(layer0 + l) * a.n_kv + g;
-    const size_t row = a.list[lg * a.budget + j], to = (size_t)a.dst_start + j;
+    // in the range whatever the list holds after such a race
+    const size_t row = min(max(a.list[lg * a.budget + j], a.start), a.start + a.len - 1), to = (size_t)a.dst_start + j;
     const int col = g * hd + 8 * c;
     const u4 kk = *(const u4*)(p.k[l] + row * sk + col), vv = *(const u4*)(p.v[l] + row * sv + col);
     *(u4*)(p.dk[l] + to * dk + col) = kk;
@@ -324,12 +326,18 @@ int gllm_hip_kv_keep_dev(const gllm_hip_kv* src, gllm_hip_kv* dst, int n_kv_head
     };
     if (!apart(d_mass, d_mass_out) || !apart(d_mass, d_pos_out) || !apart(d_pos, d_mass_out) || !apart(d_pos, d_pos_out))
         return fail(GLLM_EINVAL, "%s: outputs overlap the inputs", what);
-    GLLM_TRY(current_is(what, src));
-    GLLM_TRY(current_is(what, dst));
-    hipStream_t s = (hipStream_t)stream;
     const size_t bytes = gllm_hip_kv_keep_bytes(src->layers, n_kv_heads, budget);
     if (d_work && (((uintptr_t)d_work & 15) || work_bytes < bytes))
         return fail(GLLM_EINVAL, "%s: the workspace needs %zu bytes, 16-byte aligned", what, bytes);
+    const auto off_work = [&](const void* p, int row) {
+        const uintptr_t w = (uintptr_t)d_work, t = (uintptr_t)p;
+        return !p || !d_work || w + bytes <= t || t + heads * row * 4 <= w;
+    };
+    if (!off_work(d_mass, stride) || !off_work(d_pos, stride) || !off_work(d_mass_out, out_stride) || !off_work(d_pos_out, out_stride))
+        return fail(GLLM_EINVAL, "%s: the workspace overlaps the tensors", what);
+    GLLM_TRY(current_is(what, src));
+    GLLM_TRY(current_is(what, dst));
+    hipStream_t s = (hipStream_t)stream;
     int32_t* list = d_work ? (int32_t*)d_work : (int32_t*)thread_scratch(11, bytes, s);
     if (!list) return scratch_error();
     KeepArgs a{d_mass, d_pos, d_mass_out, d_pos_out, list, n_kv_heads, stride, out_stride, start, dst_start, len, budget, sinks,

@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 
 import gopherllm_amd as g
-from gopherllm_amd import api
+from gopherllm_amd import _lib, api
 
 
 class Torch(types.SimpleNamespace):
@@ -306,3 +306,31 @@ def test_an_empty_workspace_is_refused(calls):
         assert not calls
         getattr(cache(), name)(*lead, **args, work=Tensor(64, kind="uint8"))
         assert calls.pop()[-3:] == (4096, 64, 77)
+
+
+P = 1 << 24  # addresses that are never read: 2 layers x 2 heads x 100 rows of mass from here on
+
+
+@pytest.mark.parametrize("at", [P, P + 1596, P + (1 << 20) + 1584, P + (2 << 20) - 304, P + (2 << 20), P + (3 << 20), P + (3 << 20) + 464])
+def test_keep_refuses_a_workspace_over_its_tensors(at):
+    """The workspace holds the rows to copy: written over, they would be any rows."""
+    src, dst = cache(), cache(rows=30)
+    mass, pos, mass_out, pos_out = (C.c_void_p(P + (i << 20)) for i in range(4))
+    size = g.keep_bytes(2, 2, 20)
+    at = at // 16 * 16
+    rc = g.load().gllm_hip_kv_keep_dev(C.c_void_p(src.handle), C.c_void_p(dst.handle), 2, 64, 0, 50, 0, 20, 1, 2, 50, mass, pos, 100, mass_out,
+                                       pos_out, 30, C.c_void_p(at), size, None)
+    assert rc == g.EINVAL and "overlaps" in _lib.last_error()
+
+
+def test_keep_takes_a_workspace_next_to_its_tensors():
+    """Refused for want of a device only, not for its place."""
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("a device would run it")
+    src, dst = cache(), cache(rows=30)
+    mass, pos, mass_out, pos_out = (C.c_void_p(P + (i << 20)) for i in range(4))
+    for at in (P - 320, P + 1600, P + (2 << 20) - 320, P + (3 << 20) + 480):
+        rc = g.load().gllm_hip_kv_keep_dev(C.c_void_p(src.handle), C.c_void_p(dst.handle), 2, 64, 0, 50, 0, 20, 1, 2, 50, mass, pos, 100, mass_out,
+                                           pos_out, 30, C.c_void_p(at), g.keep_bytes(2, 2, 20), None)
+        assert rc != g.OK and "overlap" not in _lib.last_error()
