@@ -1,6 +1,7 @@
 """Accumulated attention weights where scores are far from zero, of any sign or
-all alike, against the definition in 64 bits; the tolerances are those of
-test_gpu_cache_ops.py, whose score bound S counts the offset."""
+all alike, against the definition in 64 bits (the tolerances are those of
+test_gpu_cache_ops.py, whose score bound S counts the offset); a cache's rows as
+tensors; and batches with padding."""
 import numpy as np
 import pytest
 
@@ -70,3 +71,47 @@ def test_tensors_are_the_caches_rows(hip):
         torch.cuda.synchronize()
         rk, rv = kv.read(l, 0, 9)
         assert (rk.view(np.float16) == 1.5 + l).all() and (rv.view(np.float16) == -2.0 - l).all()
+
+
+@pytest.mark.parametrize("n,heads,n_kv,hd,length", [(3, 8, 2, 64, 200), (9, 40, 8, 80, 257), (33, 32, 8, 128, 700), (70, 32, 8, 128, 129)])
+@pytest.mark.parametrize("pad", [NAN, float("inf"), -float("inf"), 3e38])
+def test_shared_padded_batch(hip, n, heads, n_kv, hd, length, pad):
+    """What stands in the queries of a batch's padding, and rows of `out` behind the batch, concern nobody."""
+    import torch
+    kv, _, _ = make_cache(hip, length + 5 * n, n_kv * hd, 1200)
+    live = np.arange(n) % 3 != 1
+    lens = cuda(np.where(live, 1 + np.arange(n) % 5, 0).astype(np.int32))
+    starts = cuda((length + 5 * np.arange(n)).astype(np.int32))
+    q = normal(1201, (n, heads * hd))
+    outs = []
+    print(f"padded batch: {n} of {heads}/{n_kv}x{hd}, {pad}", flush=True)
+    for fill in (0.0, pad):
+        q[~live] = fill
+        out = torch.full((n + 2, heads * hd), 7.0, device="cuda")
+        kv.attend_shared_dev(0, cuda(q), heads, n_kv, hd, 0, length, starts, lens, 5, hd ** -0.5, out)
+        outs.append(host(out))
+    assert np.isfinite(outs[0]).all()
+    assert np.array_equal(outs[0][:n][live], outs[1][:n][live]) and (outs[1][n:] == 7.0).all()
+
+
+@pytest.mark.parametrize("layout,rot", [("half", 64), ("interleaved", 64), ("half", 20), ("interleaved", 22)])
+def test_rope_padded_batch(hip, layout, rot):
+    """Padding (row -1) of NaN at any position stores nothing and leaves the others as they are without it."""
+    rope, n, hd = hip.Rope(64, rot_dim=rot, layout=layout), 9, 64
+    live = np.arange(n) % 3 != 1
+    q, k, v = (normal(1210 + i, (n, 2 * hd)) for i in range(3))
+    pos, rows = np.arange(n, dtype=np.int32) * 1000, np.where(live, np.arange(n), -1).astype(np.int32)
+    got = []
+    for keep in (np.ones(n, bool), live):
+        kv = hip.KVCacheF16(1, 2 * hd, 2 * hd, n + 1)
+        a, b, c = (x.copy() for x in (q, k, v))
+        for x in (a, b, c):
+            x[~keep] = NAN
+        p = np.where(keep, pos, -(2**31)).astype(np.int32)
+        dq = cuda(a)
+        kv.store_rope_dev(0, rope, dq, cuda(b), cuda(c), cuda(p), cuda(rows))
+        got.append((host(dq)[live], *(host(t) for t in kv.tensors(0))))
+    for x, y in zip(*got):
+        assert np.array_equal(x, y)
+    for t in got[1][1:]:
+        assert (t[np.r_[~live, True]] == 0).all() and (t[np.r_[live, False]] != 0).any()
