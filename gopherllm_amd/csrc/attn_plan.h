@@ -197,7 +197,10 @@ inline TreePlan tree_plan(int n, int m, int n_heads, int n_kv, int hd, int most)
     p.pw = p.rw < kSeqWaves ? 4 : p.nq == 2 || (per_kv > 64 && ranges * n_kv < 128) ? 2 : 1;
     const int workgroups = p.rw * p.pw > kSeqWaves ? kSeqTarget / 2 : kSeqTarget;  // of eight waves, of four
     p.target = std::max(1, workgroups / n_kv);
-    const long long share = std::max(1LL, (n > 1 ? kTreeSpread : 1) * (long long)p.target / ranges);
+    // and no more than the room below is for, which counts where a workgroup for each kv
+    // head is more than are wanted: past kSeqTarget of them
+    const long long share = std::max(1LL, std::min((n > 1 ? kTreeSpread : 1) * (long long)p.target / ranges,
+                                                   (long long)kTreeSpread * kSeqTarget / (ranges * n_kv)));
     p.splits = (int)std::min({(long long)kSeqMaxSplits, share, (long long)ceil_div(positions, kSeqQuantum)});
     if (whole) p.splits = 1;
     p.units = (int)std::min(p.target + ranges, ranges * p.splits);

@@ -86,6 +86,35 @@ def test_the_tree_plan_covers_every_row_and_its_room_never_falls(tmp_path):
     run(tmp_path, PLAN)
 
 
+MANY_KV_HEADS = r"""
+#include <cstdio>
+#include "attn_plan.h"
+using namespace gllm;
+int main() {
+    const int gs[] = {255, 256, 257, 511, 512, 513, 514, 534, 600, 1023, 1024, 1025, 4096}, rs[] = {1, 2, 3, 16, 32}, ns[] = {1, 2, 3, 4, 5, 8, 1000};
+    const int ms[] = {1, 4, 15, 16, 17, 64, 65, 256}, mosts[] = {0, 128, 300, 497, 1000, 4001, 32768, 1 << 30, 2147483647};
+    for (int hd : {8, 64, 128}) for (int g : gs) for (int r : rs) for (int n : ns) for (int m : ms) {
+        if ((long long)n * m * r * g > (1 << 22) || (long long)m * r > (1 << 20)) continue;
+        size_t before = 0;
+        for (int most : mosts) {
+            const TreePlan p = tree_plan(n, m, r * g, g, hd, most);
+            // the outputs, bases and sums of all parts, and each request's number of parts behind them
+            const size_t end = p.rows * (size_t)p.splits * (hd + 2) + n, room = tree_floats(p, n, hd);
+            if (p.rows * (size_t)p.splits > p.parts || end > room || room < before || p.splits < 1 || p.splits > kSeqMaxSplits ||
+                p.units > (long long)n * p.row_blocks * p.splits || (long long)g * p.units >= 1 << 23)
+                return std::printf("n %d m %d heads %d/%d of %d most %d: %zu rows of %d parts, room for %zu\n", n, m, r * g, g, hd, most, p.rows, p.splits, p.parts), 1;
+            before = room;
+        }
+    }
+}
+"""
+
+
+def test_parts_fit_their_room_for_any_number_of_kv_heads(tmp_path):
+    """A workgroup for each kv head is more than are wanted from 512 kv heads on."""
+    run(tmp_path, MANY_KV_HEADS)
+
+
 COPY = r"""
 #include <cstdio>
 #include <cstdlib>
