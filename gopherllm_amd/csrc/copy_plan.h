@@ -43,7 +43,7 @@ inline CopyPlan copy_plan(const int32_t* m, int n, bool same) {
     // move i reads rows that move j writes: i goes before j.  The destinations are
     // sorted and apart, so those that a source meets lie together.
     const int k = (int)p.moves.size();
-    std::vector<std::vector<int>> after(k);
+    std::vector<std::vector<int>> after(k), before(k);
     std::vector<int> waits(k, 0);
     bool any = false;
     for (int i = 0; i < k; i++) {
@@ -58,25 +58,36 @@ inline CopyPlan copy_plan(const int32_t* m, int n, bool same) {
             any = true;
             if (j == i) continue;  // over its own rows: copied from the right end
             after[i].push_back(j);
+            before[j].push_back(i);
             waits[j]++;
         }
     }
     if (!any) return p;
     p.apart = false;
     std::vector<RowMove> order;
-    std::vector<int> ready;
+    std::vector<int> ready, seen(k, -1);
     std::vector<bool> done(k, false);
     for (int i = 0; i < k; i++)
         if (!waits[i]) ready.push_back(i);
+    int first = 0;  // all before it are done
     for (size_t at = 0, left = k; left; left--) {
         int i;
         if (at < ready.size()) {
             i = ready[at++];
             order.push_back(p.moves[i]);
-        } else {  // the rest go round in circles: the shortest is set aside, and its rows are free
-            i = -1;
-            for (int j = 0; j < k; j++)
-                if (!done[j] && (i < 0 || p.moves[j].rows < p.moves[i].rows)) i = j;
+        } else {
+            // The rest wait for circles or are in one.  Up from one of them to what it waits
+            // for, until a move comes again: its circle's shortest is set aside, so its rows are free.
+            while (done[first]) first++;
+            const auto up = [&](int j) {
+                while (done[before[j].back()]) before[j].pop_back();
+                return before[j].back();
+            };
+            int j = first;
+            for (; seen[j] != (int)left; j = up(j)) seen[j] = (int)left;
+            i = j;
+            for (int c = up(j); c != j; c = up(c))
+                if (p.moves[c].rows < p.moves[i].rows) i = c;
             p.staged.push_back(p.moves[i]);
         }
         done[i] = true;

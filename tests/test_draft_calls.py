@@ -189,6 +189,80 @@ def test_rows_are_read_before_they_are_written(tmp_path):
     run(tmp_path, COPY)
 
 
+CIRCLES = r"""
+#include <cstdio>
+#include <random>
+#include "copy_plan.h"
+using namespace gllm;
+// Whether move x is on a circle of moves, each of which writes rows that the next reads
+static bool on_circle(const std::vector<RowMove>& all, const RowMove& x) {
+    const auto before = [](const RowMove& a, const RowMove& b) { return a.src < b.dst + b.rows && b.dst < a.src + a.rows; };
+    std::vector<char> seen(all.size(), 0);
+    std::vector<RowMove> now{x};
+    while (!now.empty()) {
+        const RowMove a = now.back();
+        now.pop_back();
+        for (size_t i = 0; i < all.size(); i++) {
+            if (all[i].dst == a.dst || !before(a, all[i])) continue;  // destinations tell moves apart
+            if (all[i].dst == x.dst) return true;
+            if (!seen[i]++) now.push_back(all[i]);
+        }
+    }
+    return false;
+}
+static long rows_of(const std::vector<RowMove>& v) {
+    long n = 0;
+    for (const RowMove& x : v) n += x.rows;
+    return n;
+}
+int main() {
+    // places 0 and 1 of 1000 rows exchanged, and moves of fewer rows that wait for them and for each other
+    for (int waiting : {0, 1, 2, 18, 300})
+        for (int less : {1, 499, 999}) {
+            std::vector<int32_t> m{0, 1000, 1000, 1000, 0, 1000};
+            for (int i = 0; i < waiting; i++) m.insert(m.end(), {1000 * (i + 2), i ? 1000 * (i + 1) : 500, less < 500 || i ? less : 500});
+            if (waiting) m[5] = 500;  // the first of them goes to rows that the exchange reads
+            const CopyPlan p = copy_plan(m.data(), (int)m.size() / 3, true);
+            const long least = waiting ? 500 : 1000;
+            if (!p.ok || p.staged.size() != 1 || rows_of(p.staged) != least) return std::printf("%d waiting: %zu moves of %ld rows set aside, not %ld\n", waiting, p.staged.size(), rows_of(p.staged), least), 1;
+        }
+    // any moves of places, some of several to one source
+    std::mt19937 rng(7);
+    long circles = 0, none = 0;
+    for (int trial = 0; trial < 3000; trial++) {
+        const int n = 2 + (int)(rng() % 30);
+        std::vector<int32_t> m;
+        for (int i = 0; i < n; i++) {
+            const int rows = 1 + (int)(rng() % 9), at = (int)(rng() % (unsigned)n);
+            m.insert(m.end(), {10 * at + (int)(rng() % (unsigned)(10 - rows + 1)), 10 * i, rows});
+        }
+        const CopyPlan p = copy_plan(m.data(), n, true);
+        std::vector<RowMove> all = p.moves;
+        all.insert(all.end(), p.staged.begin(), p.staged.end());
+        bool any = false;
+        for (const RowMove& x : all) any |= on_circle(all, x);
+        for (const RowMove& x : p.staged)
+            if (!on_circle(all, x)) return std::printf("trial %d: rows %d of %d moves set aside, in no circle\n", trial, x.rows, n), 1;
+        if (any == p.staged.empty()) return std::printf("trial %d: circles %d, %zu set aside\n", trial, (int)any, p.staged.size()), 1;
+        (any ? circles : none)++;
+    }
+    if (circles < 300 || none < 300) return std::printf("%ld %ld\n", circles, none), 1;
+    // as many moves as a call takes: one circle of all, and circles of two
+    std::vector<int32_t> ring, pairs;
+    for (int i = 0; i < kCopyMost; i++) {
+        ring.insert(ring.end(), {4 * i, 4 * ((i + 1) % kCopyMost), i == 77 ? 3 : 4});
+        pairs.insert(pairs.end(), {4 * i, 4 * (i ^ 1), 4});
+    }
+    const CopyPlan p = copy_plan(ring.data(), kCopyMost, true), q = copy_plan(pairs.data(), kCopyMost, true);
+    if (rows_of(p.staged) != 3 || q.staged.size() != kCopyMost / 2) return std::printf("%ld rows, %zu moves\n", rows_of(p.staged), q.staged.size()), 1;
+}
+"""
+
+
+def test_only_rows_of_a_circle_are_set_aside(tmp_path):
+    run(tmp_path, CIRCLES)
+
+
 # --- refusals -----------------------------------------------------------------
 
 TREE = dict(kv=None, l=0, q=P, n=3, m=4, heads=8, kvh=2, hd=64, starts=P, lens=P, most=10, parents=P, counts=P, scale=0.1, out=P,
