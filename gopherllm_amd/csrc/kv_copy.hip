@@ -204,9 +204,9 @@ static int launch_apart(const std::vector<RowMove>& all, const CopyPtrs& p, int 
 }
 
 static int order_slices(int cols, int ck, int cv) { return (ck + cols - 1) / cols + (cv + cols - 1) / cols; }
-// Whole lines where that makes workgroups enough
+// Whole lines where that makes workgroups enough for launches of `layers` layers
 static int order_cols(int layers, int ck, int cv) {
-    return (long long)std::min(layers, kCopyLayers) * order_slices(8, ck, cv) >= 2 * kOrderWorkgroups ? 8 : 4;
+    return (long long)layers * order_slices(8, ck, cv) >= 2 * kOrderWorkgroups ? 8 : 4;
 }
 
 static int launch_ordered(const std::vector<RowMove>& moves, const CopyPtrs& p, int layers, int ck, int cv, int cols, hipStream_t s) {
@@ -229,12 +229,22 @@ static int launch_ordered(const std::vector<RowMove>& moves, const CopyPtrs& p, 
     return GLLM_OK;
 }
 
-// Layers that a workspace of about 256 MB holds the rows of, one at least.
-static int staged_layers(int layers, size_t layer_bytes) {
-    return (int)std::max<size_t>(1, std::min<size_t>((size_t)std::min(layers, kCopyLayers), ((size_t)256 << 20) / layer_bytes));
+// Layers of a launch, about the same for each: as many as its arguments have room for
+// and, where rows are set aside, a workspace of about 256 MB, one at least.
+static int launch_layers(int layers, size_t staged_bytes) {
+    size_t most = std::min(layers, kCopyLayers);
+    if (staged_bytes) most = std::max<size_t>(1, std::min(most, ((size_t)256 << 20) / staged_bytes));
+    const int launches = (layers + (int)most - 1) / (int)most;
+    return (layers + launches - 1) / launches;
 }
 
-static int copy_check(const char* what, const gllm_hip_kv* src, const gllm_hip_kv* dst, const int32_t* moves, int n, CopyPlan* p, size_t* bytes) {
+struct CopyWay {
+    CopyPlan plan;
+    size_t rows, layer;  // set aside, and their bytes in a layer
+    int step, cols;      // layers of a launch; pieces of a row that a workgroup has in order
+};
+
+static int copy_check(const char* what, const gllm_hip_kv* src, const gllm_hip_kv* dst, const int32_t* moves, int n, CopyWay* way, size_t* bytes) {
     if (n < 0 || n > kCopyMost) return fail(GLLM_EINVAL, "%s: %d moves, up to %d are taken", what, n, kCopyMost);
     if (!src || !dst || (n > 0 && !moves)) return fail(GLLM_EINVAL, "%s: null pointer", what);
     if (src->layers != dst->layers || src->kv_dim_k != dst->kv_dim_k || src->kv_dim_v != dst->kv_dim_v)
@@ -248,29 +258,40 @@ static int copy_check(const char* what, const gllm_hip_kv* src, const gllm_hip_k
         rows += (size_t)m[2];
     }
     if (rows > (size_t)1 << 28) return fail(GLLM_EUNSUP, "%s: %zu rows", what, rows);
+    CopyPlan& p = way->plan;
+    const int ck = src->kv_dim_k / 8, cv = src->kv_dim_v / 8;
+    const auto lay_out = [&] {
+        way->rows = 0;
+        for (const RowMove& m : p.staged) way->rows += m.rows;
+        way->layer = way->rows * ((size_t)src->kv_dim_k + src->kv_dim_v) * 2;
+        way->step = launch_layers(src->layers, way->layer);
+        way->cols = order_cols(way->step, ck, cv);
+    };
     try {
-        *p = copy_plan(moves, n, src == dst);
-        const int cols = order_cols(src->layers, src->kv_dim_k / 8, src->kv_dim_v / 8);
-        if (!p->apart && rows <= (size_t)order_rows(cols) && p->moves.size() + p->staged.size() <= kCopyRanges) {
+        p = copy_plan(moves, n, src == dst);
+        if (!p.ok) return fail(GLLM_EINVAL, "%s: two moves write the same rows", what);
+        const int once = order_cols(launch_layers(src->layers, 0), ck, cv);
+        if (!p.apart && rows <= (size_t)order_rows(once) && p.moves.size() + p.staged.size() <= kCopyRanges) {
             // all rows are read before one is written
-            p->moves.insert(p->moves.end(), p->staged.begin(), p->staged.end());
-            p->staged.clear();
-        } else if (!p->apart && rows > (size_t)4 * order_rows(4) &&
-                   (long long)src->layers * order_slices(8, src->kv_dim_k / 8, src->kv_dim_v / 8) < kOrderWorkgroups) {
+            p.moves.insert(p.moves.end(), p.staged.begin(), p.staged.end());
+            p.staged.clear();
+        }
+        lay_out();
+        if (!p.apart && rows > (size_t)4 * order_rows(4) && (long long)way->step * order_slices(8, ck, cv) < kOrderWorkgroups) {
             // many rows twice, by all of the device, rather than in order by a few of its
             // CUs: 12000 rows of 8 heads of 128 take 50 us in order and 30 staged in one
-            // layer, 99 and 77 in two, 137 and 160 in four; 700 rows 8 and 12
-            p->staged.insert(p->staged.end(), p->moves.begin(), p->moves.end());
-            p->moves.clear();
+            // layer, 99 and 77 in two, 137 and 160 in four; 700 rows 8 and 12.  What counts
+            // is the layers of a launch: two places of 65536 such rows exchanged in 24
+            // layers, one a launch, 22.6 and 9.9 ms; 12000 rows of one head of 128 moved
+            // down by 5 in 33, 17 a launch, 0.18 and 0.11
+            p.staged.insert(p.staged.end(), p.moves.begin(), p.moves.end());
+            p.moves.clear();
+            lay_out();
         }
     } catch (const std::bad_alloc&) {
         return fail(GLLM_ENOMEM, "%s: no host memory for %d moves", what, n);
     }
-    if (!p->ok) return fail(GLLM_EINVAL, "%s: two moves write the same rows", what);
-    size_t staged = 0;
-    for (const RowMove& m : p->staged) staged += m.rows;
-    const size_t layer = staged * ((size_t)src->kv_dim_k + src->kv_dim_v) * 2;
-    *bytes = layer ? layer * staged_layers(src->layers, layer) : 0;
+    *bytes = way->layer * way->step;
     return GLLM_OK;
 }
 
@@ -302,17 +323,18 @@ int gllm_hip_kv_keep_path_dev(gllm_hip_kv* kv, int n, int m, const int32_t* d_st
 }
 
 size_t gllm_hip_kv_copy_rows_bytes(const gllm_hip_kv* src, const gllm_hip_kv* dst, const int32_t* moves, int n) {
-    CopyPlan p;
+    CopyWay way;
     size_t bytes = 0;
-    return copy_check("gllm_hip_kv_copy_rows_bytes", src, dst, moves, n, &p, &bytes) == GLLM_OK ? bytes : 0;
+    return copy_check("gllm_hip_kv_copy_rows_bytes", src, dst, moves, n, &way, &bytes) == GLLM_OK ? bytes : 0;
 }
 
 int gllm_hip_kv_copy_rows_dev(const gllm_hip_kv* src, gllm_hip_kv* dst, const int32_t* moves, int n, void* d_work, size_t work_bytes,
                               void* stream) {
     const char* what = "gllm_hip_kv_copy_rows_dev";
-    CopyPlan plan;
+    CopyWay way;
     size_t bytes = 0;
-    GLLM_TRY(copy_check(what, src, dst, moves, n, &plan, &bytes));
+    GLLM_TRY(copy_check(what, src, dst, moves, n, &way, &bytes));
+    const CopyPlan& plan = way.plan;
     GLLM_TRY(copy_current(what, src));
     GLLM_TRY(copy_current(what, dst));
     if (d_work && (((uintptr_t)d_work & 15) || work_bytes < bytes))
@@ -339,17 +361,15 @@ int gllm_hip_kv_copy_rows_dev(const gllm_hip_kv* src, gllm_hip_kv* dst, const in
             in.push_back({(int)rows, m.dst, m.rows});
             rows += m.rows;
         }
-        const size_t layer = rows * ((size_t)ck + cv) * 16;
-        const int step = bytes ? staged_layers(src->layers, layer) : kCopyLayers;
-        for (int l0 = 0; l0 < src->layers; l0 += step) {
-            const int layers = std::min(step, src->layers - l0);
+        for (int l0 = 0; l0 < src->layers; l0 += way.step) {
+            const int layers = std::min(way.step, src->layers - l0);
             CopyPtrs p{}, there{}, back{};
             for (int i = 0; i < layers; i++) {
                 p.k[i] = there.k[i] = src->k[l0 + i];
                 p.v[i] = there.v[i] = src->v[l0 + i];
                 p.dk[i] = back.dk[i] = dst->k[l0 + i];
                 p.dv[i] = back.dv[i] = dst->v[l0 + i];
-                uint16_t* at = (uint16_t*)(work + layer * i);
+                uint16_t* at = (uint16_t*)(work + way.layer * i);
                 back.k[i] = there.dk[i] = at;
                 back.v[i] = there.dv[i] = at + rows * ck * 8;
             }
@@ -358,7 +378,7 @@ int gllm_hip_kv_copy_rows_dev(const gllm_hip_kv* src, gllm_hip_kv* dst, const in
                 continue;
             }
             GLLM_TRY(launch_apart(out, there, layers, ck, cv, s));
-            GLLM_TRY(launch_ordered(plan.moves, p, layers, ck, cv, order_cols(src->layers, ck, cv), s));
+            GLLM_TRY(launch_ordered(plan.moves, p, layers, ck, cv, way.cols, s));
             GLLM_TRY(launch_apart(in, back, layers, ck, cv, s));
         }
     } catch (const std::bad_alloc&) {

@@ -355,6 +355,30 @@ def test_workspace_sizes():
     assert staged(moves((0, 1000, 1000), (1000, 2000, 1000)), **few) == 0 and staged(moves((0, 5000, 1000)), **few) == 0 and staged(moves((5, 0, 500)), **few) == 0
 
 
+def test_what_goes_in_order_is_decided_by_the_layers_of_a_launch():
+    """Workgroups own 128 bytes of a layer's rows: fewer than 96 of them in a launch read many rows twice."""
+    def staged(m, rows, **kw):
+        a = cache(rows=rows, **kw)
+        return g.load().gllm_hip_kv_copy_rows_bytes(C.byref(a), C.byref(a), m.ctypes.data_as(C.c_void_p), len(m))
+
+    def exchange(n):
+        return moves((0, n, n), (n, 0, n))
+    row = (1024 + 1024) * 2
+    many = dict(layers=24, kd=1024, vd=1024)
+    assert staged(exchange(40000), 80000, **many) == 80000 * row  # in order: one layer a launch, so all of its rows
+    assert staged(exchange(32768), 65536, **many) == 65536 * row  # two
+    assert staged(exchange(20000), 40000, **many) == 3 * 20000 * row  # three are enough
+    shift = moves((5, 0, 5000))
+    assert staged(shift, 5005, layers=32, kd=192, vd=192) == 0  # 32 layers of 6 workgroups
+    assert staged(shift, 5005, layers=33, kd=192, vd=192) == 0  # and 17 of 6
+    assert staged(shift, 5005, layers=32, kd=128, vd=128) == 0 and staged(shift, 5005, layers=33, kd=128, vd=128) == 17 * 5000 * 512
+    # a launch's workspace is about 256 MB, whatever goes through it
+    for n in (3000, 20000, 32768, 100000):
+        for kw in (many, dict(layers=1, kd=64, vd=64), dict(layers=80, kd=256, vd=128)):
+            layer = 2 * n * (kw["kd"] + kw["vd"]) * 2
+            assert staged(exchange(n), 2 * n, **kw) <= max(256 << 20, layer)
+
+
 def test_workspaces_over_the_tensors_are_refused():
     at = lambda x: C.c_void_p((1 << 20) + x)  # noqa: E731
     big = 1 << 30
