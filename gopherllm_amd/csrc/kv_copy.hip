@@ -48,8 +48,8 @@ __global__ __launch_bounds__(256) void keep_path_kernel(CopyPtrs p, PathArgs a) 
         for (int u = 0; u < U; u++) {
             const int k = k0 + u, j = k < taken ? path[k] : 0;
             from[u] = base + j;
-            // what is in place already, or outside the tree or the cache, stays
-            if (k >= taken || j <= k || j >= a.m || base < 0 || from[u] >= a.max_len) from[u] = -1;
+            // what is in place already, or outside the tree or the cache, or would go there, stays
+            if (k >= taken || j <= k || j >= a.m || base + k < 0 || from[u] >= a.max_len) from[u] = -1;
             if (from[u] >= 0) x[u] = rows[from[u] * per];
         }
 #pragma unroll
