@@ -322,7 +322,9 @@ struct TreeLds {
 // with both parts) take 69 us, 1.0 PFLOP/s where a large library product reaches 1.15;
 // the cores are busy 52 % of the waves' time, LDS 15 %, without a bank conflict.
 // Two stages are enough, as the steps of a CU's waves do not run in time with each
-// other: rings of three and four measured the same and leave a CU fewer waves.  Short
+// other: rings of three and four measured the same.  With 16 rows a wave they would also
+// leave a CU fewer waves; with 32 the joined sums fill LDS (128 KB for heads of 128, as
+// much as a ring of four) and a CU has one workgroup either way.  Short
 // contexts are bound by latency: 33 tokens over 4001 rows take 17 us, seven steps of
 // about 1 us and the rest the start (lengths, queries, first tiles) and the end (sums
 // joined in LDS, partial results written).  One step's latency is K's reads, 8 products in a row, exponentials, V's reads and
@@ -330,7 +332,8 @@ struct TreeLds {
 template <int HD, int NQ, int RW, int PW, int ST>
 __global__ __launch_bounds__(64 * RW * PW, 2) void tree_attend_kernel(TreeArgs t) {
     constexpr int DT = HD / 16, CH = HD / 8, TILE = kStep * HD * 2, STAGE = TreeLds<HD, NQ, RW, PW, ST>::STAGE;
-    constexpr int COPIES = 2 * kStep * CH / 64, U = (COPIES + RW - 1) / RW;  // copies of a stage, 64 chunks each, and of a wave
+    constexpr int COPIES = 2 * kStep * CH / 64, U = COPIES / RW;  // copies of a stage, 64 chunks each, and of a wave
+    static_assert(COPIES % RW == 0, "as many copies for each wave");
     static_assert(64 * RW * PW >= kTreeTokens, "a token a thread");
     __shared__ __align__(16) char lds[TreeLds<HD, NQ, RW, PW, ST>::BYTES];
     __shared__ TreeSeen seen;
@@ -382,7 +385,7 @@ __global__ __launch_bounds__(64 * RW * PW, 2) void tree_attend_kernel(TreeArgs t
     int off[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const int c = (RW * u + rw) % COPIES;  // of the stage; where they do not come out even, one is made twice
+        const int c = RW * u + rw;  // of the stage
         const bool v = c >= COPIES / 2;
         const int e = 64 * (v ? c - COPIES / 2 : c) + lane, rr = e / CH, d = 8 * (e % CH ^ (v ? v_swizzle<HD>(rr) : k_swizzle<HD>(rr)));
         off[u] = d < t.hd ? (rr * (v ? t.kd_v : t.kd_k) + d) * 2 : kPastEnd;
@@ -395,7 +398,7 @@ __global__ __launch_bounds__(64 * RW * PW, 2) void tree_attend_kernel(TreeArgs t
         const uint32_t to = ring_at + (step % ST) * STAGE;
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int c = (RW * u + rw) % COPIES;
+            const int c = RW * u + rw;
             lds_buffer16(c >= COPIES / 2 ? v : k, off[u], to + 1024 * c);
         }
     };
