@@ -325,7 +325,7 @@ struct TreeLds {
 // other: rings of three and four measured the same.  With 16 rows a wave they would also
 // leave a CU fewer waves; with 32 the joined sums fill LDS (128 KB for heads of 128, as
 // much as a ring of four) and a CU has one workgroup either way.  Short
-// contexts are bound by latency: 33 tokens over 4001 rows take 17 us, seven steps of
+// contexts are bound by latency: 33 tokens over 4001 rows take 16 to 18 us, seven steps of
 // about 1 us and the rest the start (lengths, queries, first tiles) and the end (sums
 // joined in LDS, partial results written).  One step's latency is K's reads, 8 products in a row, exponentials, V's reads and
 // products; starting the next step's reads under them took registers and no time off.

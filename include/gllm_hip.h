@@ -408,7 +408,7 @@ int gllm_hip_attend_tree_dev(gllm_hip_kv* kv, int l, const float* d_q, int n, in
 /* The drafted tokens that the model agrees with.  d_logits: n * m rows of vocab
  * floats, stride apart.  The choice after a token is its largest finite logit
  * (temperature 0; the lowest token on ties, 0 where none is finite: the choice of
- * gllm_hip_argmax_dev), or, with d_uniforms [n][m] in [0, 1), a sample: the first
+ * gllm_hip_argmax_dev, without a repeat penalty), or, with d_uniforms [n][m] in [0, 1), a sample: the first
  * token at which the sum of exp(logit / temperature) over finite logits passes
  * uniform * the whole sum, in 64 bits.  From token 0 on, the path goes on to the
  * child that holds the choice (of several, the first).  d_path [n][m]: the path's
@@ -423,9 +423,10 @@ int gllm_hip_accept_tree_dev(const float* d_logits, int stride, int vocab, int n
                              size_t work_bytes, void* stream);
 /* The rows of the accepted tokens moved together, in every layer: row d_starts[i]
  * + d_lens[i] + d_path[i][k] goes to row d_starts[i] + d_lens[i] + k for k <
- * d_accepted[i].  d_path [n][m] goes up from at least 0 (an entry <= k, >= m or
- * outside the cache moves nothing); the requests' rows do not overlap (n up to
- * 65535).  The context's new length is d_lens[i] + d_accepted[i]: the caller's to add. */
+ * d_accepted[i].  d_path [n][m] goes up from at least 0 (an entry <= k or >= m moves
+ * nothing, nor does one whose row, or the row it goes to, is outside the cache); the
+ * requests' rows do not overlap (n up to 65535; kv_dim % 8 == 0, as for the copies).
+ * The context's new length is d_lens[i] + d_accepted[i]: the caller's to add. */
 int gllm_hip_kv_keep_path_dev(gllm_hip_kv* kv, int n, int m, const int32_t* d_starts,
                               const int32_t* d_lens, const int32_t* d_path,
                               const int32_t* d_accepted, void* stream);
@@ -434,8 +435,9 @@ int gllm_hip_kv_keep_path_dev(gllm_hip_kv* kv, int n, int m, const int32_t* d_st
  * rows (host memory, read during the call), as if all rows were read before one
  * is written: sources may overlap each other and destinations, as when requests
  * move down over free rows or exchange places; destinations must not overlap each
- * other.  Where moves write what others read, some rows may go through a workspace,
- * of the bytes that _bytes says (0: none); up to 2^28 rows. */
+ * other.  Where moves write what they or others read, as a plain shift does, some or all
+ * rows may go through a workspace, of the bytes that _bytes says (0: none; moves that
+ * write nothing that any reads need none); up to 2^28 rows. */
 size_t gllm_hip_kv_copy_rows_bytes(const gllm_hip_kv* src, const gllm_hip_kv* dst,
                                    const int32_t* moves, int n);
 int gllm_hip_kv_copy_rows_dev(const gllm_hip_kv* src, gllm_hip_kv* dst, const int32_t* moves, int n,
